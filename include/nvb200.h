@@ -37,7 +37,7 @@ enum {
 };
 
 /* Element types. */
-enum { NVB200_BF16 = 0, NVB200_F16 = 1, NVB200_F32 = 2 };
+enum { NVB200_BF16 = 0, NVB200_F16 = 1, NVB200_F32 = 2, NVB200_E4M3 = 3, NVB200_I8 = 4 /* 8-bit caches only */ };
 
 /* Bits an entry point may OR into its optional device status word (int32, zero it to clear). The kernels
  * never trap: an index they cannot honour is skipped and reported here. */
@@ -329,6 +329,117 @@ NVB200_API int nvb200_paged_decode_attention_streamk(const nvb200_paged_decode_a
 #define NVB200_DECODE_NOALLOC_SCRATCH_BYTES (4 << 20)
 #define NVB200_DECODE_NOALLOC_MAX_PAIRS 16384
 NVB200_API int nvb200_paged_decode_attention_noalloc(const nvb200_paged_decode_args *args, nvb200_stream_t stream);
+
+/* An 8-bit paged KV cache. A row (one token of one KV head) is head_dim codes and one fp32 scale; its values are
+ * code * scale.
+ *   k_cache, v_cache: codes, contiguous [num_blocks, block_size, num_kv_heads, head_dim].
+ *   k_scale, v_scale: contiguous [num_blocks, num_kv_heads, block_size].
+ *   dtype NVB200_E4M3: the scale is 2^E, E the smallest integer >= -126 with max|x| <= 448 * 2^E, and a code is
+ *     x * 2^-E rounded to e4m3 (nearest even). NVB200_I8: the scale is d / 127 with d = max(max|x|, 127 * 2^-126), and a
+ *     code is 127 x / d rounded half to even.
+ *   A row that holds an infinity or NaN gets scale NaN and codes 0: it reads back as NaN throughout. */
+typedef struct nvb200_quant_cache {
+  void *k_cache;
+  void *v_cache;
+  float *k_scale;
+  float *v_scale;
+  int64_t num_blocks;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t dtype; /* NVB200_E4M3 or NVB200_I8 */
+} nvb200_quant_cache;
+
+/* nvb200_store_kvcache into an 8-bit cache: row h of token t of key and value ([num_kv_heads, head_dim] contiguous
+ * elements at key + t * key_token_stride) is quantised and stored at slot slot_mapping[t] (slot s is token
+ * s % block_size of block s / block_size). Slot -1 stores nothing; a slot outside [-1, num_blocks * block_size) is not
+ * stored and sets NVB200_STATUS_BAD_SLOT. The other slots of one call must differ from each other: two tokens written
+ * to one slot leave its codes and scale from different tokens. dtype: of key and value. Any head_dim and alignment;
+ * multiples of 8 up to 256 on 16-byte aligned rows take the vectorised kernel.
+ * Counterpart in the reference: nanovllm/layers/attention.py:34-41 (store_kvcache), 16-bit only. */
+NVB200_API int nvb200_store_kvcache_quant(const void *key, int64_t key_token_stride, const void *value,
+                                          int64_t value_token_stride, const void *slot_mapping, int slot_bytes,
+                                          int64_t num_tokens, int dtype, const nvb200_quant_cache *cache,
+                                          int32_t *status, nvb200_stream_t stream);
+
+/* nvb200_qk_norm_rope_kv with its cache write quantised: q_out, k_out and the bf16 rows that are quantised have the
+ * bits of that function; the rows are then stored as nvb200_store_kvcache_quant does (v raw, k normed and rotated).
+ * args: as for nvb200_qk_norm_rope_kv, its k_cache, v_cache and num_slots ignored, slot_mapping required.
+ * Takes head_dim 64, 128 and 256 with 16-byte aligned rows; NVB200_ERR_UNSUPPORTED otherwise (the caller runs
+ * nvb200_qk_norm_rope_kv without a cache, then nvb200_store_kvcache_quant).
+ * Counterpart in the reference: nanovllm/kernels/qk_norm_rope_kv.py:92-125, whose cache is 16-bit. */
+NVB200_API int nvb200_qk_norm_rope_kv_quant(const nvb200_qk_norm_rope_kv_args *args, const nvb200_quant_cache *cache,
+                                            nvb200_stream_t stream);
+
+/* Reads an 8-bit cache back into packed rows, as a variable-length prefill attention takes them: row t of key and value
+ * (contiguous [total_tokens, num_kv_heads, head_dim], 16 or 32 bits by dtype) is token t - cu_seqlens[b] of sequence b,
+ * cu_seqlens[b] <= t < cu_seqlens[b + 1], found through block_table [batch, max_blocks_per_seq] int32 (row stride
+ * block_table_stride). cu_seqlens: [batch + 1] int32, not falling. Rows outside every sequence (behind the last one)
+ * are zeroed if zero_rest is 1 and left as they are if it is 0. A token whose page lies behind the block-table row, or
+ * whose entry lies outside [0, num_blocks), is not followed: zeros, and NVB200_STATUS_BAD_SLOT.
+ * No counterpart in the reference, whose prefill attention reads the 16-bit cache directly. */
+NVB200_API int nvb200_load_kvcache_quant(void *key, void *value, const nvb200_quant_cache *cache,
+                                         const int32_t *block_table, int64_t block_table_stride,
+                                         int32_t max_blocks_per_seq, const int32_t *cu_seqlens, int32_t batch,
+                                         int64_t total_tokens, int dtype, int zero_rest, int32_t *status,
+                                         nvb200_stream_t stream);
+
+/* Attention of n = queries_per_seq new tokens per sequence over the paged cache, 16-bit or 8-bit. The last
+ * m = draft_lens[b] (NULL: n) of sequence b's seqlens[b] keys are the new tokens themselves, already written; the keys
+ * before them are the context.
+ *   tree_mask (bytes, [batch, n, n] with the given strides in bytes, 0 for a mask shared by the batch): new token i < m
+ *     sees the context, and new token j < m where tree_mask[b, i, j] != 0 (its ancestors and itself, for a tree of drafted
+ *     tokens; nothing is implied, the diagonal included).
+ *   tree_mask NULL, causal 1: the chain, token i sees new tokens 0..i. causal 0: every token sees every key.
+ * Rows of tokens i >= m, and rows that see no key, are zeros. A key that a row does not see has no effect on it,
+ * whatever its bits. Where seqlens[b] < m, the first m - seqlens[b] new tokens are not in the cache and seen by no row.
+ *   q: [batch, n, num_q_heads, head_dim] with the given strides, unit last stride; dtype bf16 or fp16.
+ *   cache_dtype: = dtype (16-bit cache, strides as given, unit last stride), or NVB200_E4M3 / NVB200_I8 with k_scale and
+ *     v_scale contiguous [num_blocks, num_kv_heads, block_size] (see nvb200_quant_cache).
+ *   block_table, seqlens, num_splits, softmax_scale, status: as for nvb200_paged_decode_attention. Keys whose block-table
+ *     entry lies outside [0, num_blocks) are seen by no row; they, lengths beyond max_blocks_per_seq * block_size
+ *     and draft_lens outside [0, n] (both clamped) set NVB200_STATUS_BAD_SLOT.
+ *   out: [batch, n, num_q_heads, head_dim] contiguous, dtype, written.
+ * Takes head_dim 64 and 128, n <= 4096 and 16-byte aligned cache rows; NVB200_ERR_UNSUPPORTED otherwise.
+ * Replaces: nothing in the reference, which verifies linear drafts through flash_attn_with_kvcache
+ * (nanovllm/layers/attention.py:84-91). */
+typedef struct nvb200_cache_attention_args {
+  void *out;
+  const void *q;
+  int64_t q_batch_stride;
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  const void *k_cache;
+  const void *v_cache;
+  int64_t cache_block_stride;
+  int64_t cache_token_stride;
+  int64_t cache_head_stride;
+  const float *k_scale;
+  const float *v_scale;
+  int64_t num_blocks;
+  const int32_t *block_table;
+  int64_t block_table_stride;
+  const int32_t *seqlens;
+  const int32_t *draft_lens;
+  const uint8_t *tree_mask;
+  int64_t mask_batch_stride;
+  int64_t mask_row_stride;
+  int32_t batch;
+  int32_t queries_per_seq;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t block_size;
+  int32_t max_blocks_per_seq;
+  int32_t causal;
+  int32_t num_splits;
+  int32_t dtype;
+  int32_t cache_dtype;
+  float softmax_scale;
+  int32_t *status;
+} nvb200_cache_attention_args;
+
+NVB200_API int nvb200_cache_attention(const nvb200_cache_attention_args *args, nvb200_stream_t stream);
 
 #ifdef __cplusplus
 }

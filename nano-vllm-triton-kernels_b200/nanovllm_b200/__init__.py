@@ -11,5 +11,10 @@ from nanovllm_b200.kernels.qk_norm_rope_kv import qk_norm_rope_kv  # noqa: F401
 from nanovllm_b200.kernels.rms_norm import fused_add_rms_norm, rms_norm  # noqa: F401
 from nanovllm_b200.kernels.matmul import matmul  # noqa: F401
 from nanovllm_b200.kernels.swiglu import silu_and_mul  # noqa: F401
+from nanovllm_b200.kernels.kv_quant import (empty_quant_cache, load_kvcache_quant, qk_norm_rope_kv_quant,  # noqa: F401
+                                            store_kvcache_quant)
+from nanovllm_b200.kernels.cache_attention import decode_attention_quant, tree_attention  # noqa: F401
 
-__all__ = ["qk_norm_rope_kv", "rms_norm", "fused_add_rms_norm", "silu_and_mul", "matmul", "status", "install"]
+__all__ = ["qk_norm_rope_kv", "rms_norm", "fused_add_rms_norm", "silu_and_mul", "matmul", "empty_quant_cache",
+           "store_kvcache_quant", "qk_norm_rope_kv_quant", "load_kvcache_quant", "decode_attention_quant",
+           "tree_attention", "status", "install"]

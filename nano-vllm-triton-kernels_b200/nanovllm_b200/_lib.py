@@ -16,6 +16,8 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libnvb200.s
 OK, ERR_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_NO_DEVICE = 0, 1, 2, 3, 4
 BF16, F16, F32 = 0, 1, 2
 DTYPE_CODE = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
+E4M3, I8 = 3, 4
+QUANT_CODE = {torch.float8_e4m3fn: E4M3, torch.int8: I8}  # element types of 8-bit caches
 STATUS_BAD_POSITION, STATUS_BAD_SLOT, STATUS_WAIT_TIMEOUT = 1, 2, 4
 # NVB200_QKNR_KERNEL_* codes of nvb200_qk_norm_rope_kv_plan.
 QKNR_KERNELS = {0: "none", 1: "generic", 2: "direct", 3: "multi", 4: "bulk"}
@@ -28,7 +30,9 @@ EXPORTS = ("nvb200_status_string", "nvb200_qk_norm_rope_kv", "nvb200_qk_norm_rop
            "nvb200_allreduce_buffer_bytes", "nvb200_allreduce_buffer_create", "nvb200_allreduce_buffer_open",
            "nvb200_allreduce_buffer_close", "nvb200_matmul_allreduce", "nvb200_store_kvcache",
            "nvb200_paged_decode_attention", "nvb200_paged_decode_splits", "nvb200_paged_decode_workspace_size",
-           "nvb200_paged_decode_attention_streamk", "nvb200_paged_decode_attention_noalloc")
+           "nvb200_paged_decode_attention_streamk", "nvb200_paged_decode_attention_noalloc",
+           "nvb200_store_kvcache_quant", "nvb200_qk_norm_rope_kv_quant", "nvb200_load_kvcache_quant",
+           "nvb200_cache_attention")
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
 
@@ -63,6 +67,28 @@ class PagedDecodeArgs(ctypes.Structure):
         ("seqlens", _vp), ("batch", _i32), ("queries_per_seq", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32),
         ("head_dim", _i32), ("block_size", _i32), ("max_blocks_per_seq", _i32), ("causal", _i32),
         ("num_splits", _i32), ("dtype", _i32), ("softmax_scale", _f32), ("status", _vp),
+    ]
+
+
+class QuantCache(ctypes.Structure):
+    """nvb200_quant_cache (field order and types as in nvb200.h)."""
+    _fields_ = [
+        ("k_cache", _vp), ("v_cache", _vp), ("k_scale", _vp), ("v_scale", _vp), ("num_blocks", _i64),
+        ("block_size", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32),
+    ]
+
+
+class CacheAttentionArgs(ctypes.Structure):
+    """nvb200_cache_attention_args (field order and types as in nvb200.h)."""
+    _fields_ = [
+        ("out", _vp), ("q", _vp), ("q_batch_stride", _i64), ("q_token_stride", _i64), ("q_head_stride", _i64),
+        ("k_cache", _vp), ("v_cache", _vp), ("cache_block_stride", _i64), ("cache_token_stride", _i64),
+        ("cache_head_stride", _i64), ("k_scale", _vp), ("v_scale", _vp), ("num_blocks", _i64), ("block_table", _vp),
+        ("block_table_stride", _i64), ("seqlens", _vp), ("draft_lens", _vp), ("tree_mask", _vp),
+        ("mask_batch_stride", _i64), ("mask_row_stride", _i64), ("batch", _i32), ("queries_per_seq", _i32),
+        ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("block_size", _i32),
+        ("max_blocks_per_seq", _i32), ("causal", _i32), ("num_splits", _i32), ("dtype", _i32), ("cache_dtype", _i32),
+        ("softmax_scale", _f32), ("status", _vp),
     ]
 
 
@@ -129,6 +155,16 @@ def _declare(lib):
     lib.nvb200_paged_decode_attention_streamk.restype = ctypes.c_int
     lib.nvb200_paged_decode_attention_noalloc.argtypes = [ctypes.POINTER(PagedDecodeArgs), _vp]
     lib.nvb200_paged_decode_attention_noalloc.restype = ctypes.c_int
+    lib.nvb200_store_kvcache_quant.argtypes = [_vp, _i64, _vp, _i64, _vp, ctypes.c_int, _i64, ctypes.c_int,
+                                               ctypes.POINTER(QuantCache), _vp, _vp]
+    lib.nvb200_store_kvcache_quant.restype = ctypes.c_int
+    lib.nvb200_qk_norm_rope_kv_quant.argtypes = [ctypes.POINTER(QkNormRopeKvArgs), ctypes.POINTER(QuantCache), _vp]
+    lib.nvb200_qk_norm_rope_kv_quant.restype = ctypes.c_int
+    lib.nvb200_load_kvcache_quant.argtypes = [_vp, _vp, ctypes.POINTER(QuantCache), _vp, _i64, _i32, _vp, _i32, _i64,
+                                              ctypes.c_int, ctypes.c_int, _vp, _vp]
+    lib.nvb200_load_kvcache_quant.restype = ctypes.c_int
+    lib.nvb200_cache_attention.argtypes = [ctypes.POINTER(CacheAttentionArgs), _vp]
+    lib.nvb200_cache_attention.restype = ctypes.c_int
 
 
 def lib():
@@ -157,6 +193,22 @@ def check(rc: int, what: str) -> None:
 def stream_of(t: torch.Tensor) -> int:
     """The current torch stream of t's device (kernels launch there, as Triton's do)."""
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+class _SameDevice:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_same_device = _SameDevice()
+
+
+def device_of(device: torch.device):
+    """A context in which `device` is the current CUDA device (the entry points launch on the current one)."""
+    return _same_device if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def ptr(t):
