@@ -17,40 +17,14 @@
 #include <atomic>
 #include <cmath>
 
-#include "common.cuh"
-#include "kv_quant_math.cuh"
+#include "cache_attention.cuh"
 
 namespace nvb200 {
 namespace {
 
-enum { kBf16 = 0, kF16 = 1, kE4M3 = 2, kI8 = 3 };  // element type of the cache
-
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;          // query rows of a CTA: the rows of one m16n8k16 instruction
-constexpr int kMaxSplits = 8;      // portable cluster size
-
-struct CacheAttnParams {
-  const void *q;
-  int64_t q_batch_stride, q_token_stride, q_head_stride;
-  const uint8_t *k_cache;
-  const uint8_t *v_cache;
-  int64_t blk_stride, tok_stride, head_stride;  // elements
-  int64_t num_blocks;
-  const float *k_scale;  // [blocks, hkv, block_size], 8-bit caches
-  const float *v_scale;
-  const int32_t *block_table;  // NULL: sequence b is block b
-  int64_t bt_stride;
-  const int32_t *seqlens;
-  const int32_t *draft_lens;  // NULL: n tokens in every sequence
-  const uint8_t *mask;        // [batch, n, n] bytes, NULL: chain (causal) or no mask
-  int64_t mask_batch_stride, mask_row_stride;
-  void *out;                  // [batch, n, hq, D] contiguous
-  int n, hq, hkv, group, block_size, bs_shift, max_pages, rows, causal, splits;
-  int q_is_f16;
-  float scale_log2;
-  int32_t *status;
-};
 
 NVB200_DEVICE void cp_async16(uint32_t dst, const void *src, uint32_t src_bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
@@ -66,31 +40,6 @@ NVB200_DEVICE float2 ld_shared_f2(uint32_t addr) {
   asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
   return v;
 }
-NVB200_DEVICE uint32_t ld_shared_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
-NVB200_DEVICE void st_shared_u32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-
-NVB200_DEVICE uint32_t cta_rank_in_cluster() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-NVB200_DEVICE uint32_t map_shared_to(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-NVB200_DEVICE void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
-NVB200_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-NVB200_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
 NVB200_DEVICE void mma_16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -98,38 +47,11 @@ NVB200_DEVICE void mma_16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-NVB200_DEVICE uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
-template <int CT> struct CacheType {
-  static constexpr bool kQuant = CT == kE4M3 || CT == kI8;
-  static constexpr int kBytes = kQuant ? 1 : 2;
-  static constexpr bool kBf16Mma = CT == kBf16;
-};
-
 template <int CT> NVB200_DEVICE void mma_ct(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (CacheType<CT>::kBf16Mma) mma_16816(d, a, b0, b1);
   else mma_16816_f16(d, a, b0, b1);
 }
 
-// Bytes 0, 1 (lo) and 2, 3 (hi) of w, codes of an 8-bit cache, as two fp16 pairs.
-template <int CT> NVB200_DEVICE void codes_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
-  if constexpr (CT == kE4M3) {
-    lo = e4m3x2_to_f16x2(static_cast<uint16_t>(w & 0xFFFFu));
-    hi = e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16));
-  } else {
-    // 0x6400 | u is the fp16 number 1024 + u, u = code + 128: subtracting 1152 leaves the code, exactly.
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
-    lo = *reinterpret_cast<const uint32_t *>(&x), hi = *reinterpret_cast<const uint32_t *>(&y);
-  }
-}
 // The same for the byte pairs (0, 2) and (1, 3).
 template <int CT> NVB200_DEVICE void codes_to_f16_even_odd(uint32_t w, uint32_t &even, uint32_t &odd) {
   codes_to_f16<CT>(__byte_perm(w, 0u, 0x3120), even, odd);
@@ -310,15 +232,6 @@ NVB200_DEVICE void fold_tile(RowState<D> &st, uint32_t kt, const uint32_t (&qa)[
   __syncwarp();  // every lane is done with this stage before it is refilled
 }
 
-// Bits of the elements of w (two 16-bit elements or four e4m3 codes) that are infinite or NaN, set over the whole
-// element. int8 codes are always finite.
-template <int CT> NVB200_DEVICE uint32_t nonfinite_bits(uint32_t w) {
-  if constexpr (CT == kI8) return 0u;
-  if constexpr (CT == kE4M3) return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-  constexpr uint32_t kExp = CT == kBf16 ? 0x7F807F80u : 0x7C007C00u;
-  return __vcmpeq2(w & kExp, kExp);
-}
-
 // Replaces every infinity and NaN of the V tile by zero; true if there were any (in any lane).
 template <int CT, int D> NVB200_DEVICE bool clean_v_tile(uint32_t kt, int lane) {
   using G = Geometry<CT, D>;
@@ -384,11 +297,10 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
   const int my_tiles = warp < ntiles ? (ntiles - warp + kWarps - 1) / kWarps : 0;
 
   const int32_t *bt = p.block_table ? p.block_table + b * p.bt_stride : nullptr;
-  auto page_of = [&](int j) { return p.bs_shift >= 0 ? j >> p.bs_shift : j / p.block_size; };
   auto key_of = [&](int i) { return js + (warp + i * kWarps) * G::kTile + (lane & (G::kTile - 1)); };
   auto block_of = [&](int j) {  // block of key j, -1 past the share
     if (j >= je) return -1;
-    return bt ? __ldg(bt + page_of(j)) : b;
+    return bt ? __ldg(bt + page_of(p, j)) : b;
   };
   int next_blk = my_tiles > 0 ? block_of(key_of(0)) : -1;
   // Copies this warp's i-th tile into ring stage `stage`; the block number of the tile after it is fetched meanwhile.
@@ -399,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
     int64_t off = -1;  // element offset of key j's row for head h; -1 = not read (zero-filled)
     int in = 0;
     if (j < je) {
-      in = j - page_of(j) * p.block_size;
+      in = j - page_of(p, j) * p.block_size;
       if (blk >= 0 && blk < p.num_blocks)
         off = blk * p.blk_stride + in * p.tok_stride + h * p.head_stride;
       else
@@ -557,24 +469,7 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
     if (qi < drafts) {
       // l > 0 wherever a key was seen; NaN (a NaN score) is passed on.
       if (x.l != 0.f) y = x.o / x.l * (C::kQuant ? exp2f(x.M - x.m) : 1.f);
-      if (CT != kI8 && x.flag != 0.f) {
-        // Infinities and NaN of V that this row does see, left out of its tiles: they decide the column.
-        for (int k = 0; k < drafts; ++k) {
-          const int j = ctx + k;
-          if (j < 0 || j >= L || !(p.mask ? p.mask[b * p.mask_batch_stride + qi * p.mask_row_stride + k] != 0 : k <= qi))
-            continue;
-          const int64_t blk = bt ? __ldg(bt + page_of(j)) : b;
-          if (blk < 0 || blk >= p.num_blocks) continue;
-          const int64_t at = blk * p.blk_stride + (j - page_of(j) * p.block_size) * p.tok_stride + h * p.head_stride + d;
-          if constexpr (C::kQuant) {
-            if ((__ldg(p.v_cache + at) & 0x7Fu) == 0x7Fu) y = __uint_as_float(0x7FC00000u);
-          } else {
-            const uint16_t u = __ldg(reinterpret_cast<const uint16_t *>(p.v_cache) + at);
-            if (nonfinite_bits<CT>(u))
-              y += CT == kBf16 ? __uint_as_float(static_cast<uint32_t>(u) << 16) : __half2float(__ushort_as_half(u));
-          }
-        }
-      }
+      if (CT != kI8 && x.flag != 0.f) y = add_nonfinite<CT>(p, bt, b, h, qi, d, ctx, L, drafts, y);
     }
     const int64_t idx = ((static_cast<int64_t>(b) * p.n + qi) * p.hq + h * p.group + gq) * D + d;
     if (C::kQuant ? p.q_is_f16 : CT == kF16) static_cast<__half *>(p.out)[idx] = __float2half_rn(y);
@@ -705,6 +600,10 @@ extern "C" int nvb200_cache_attention(const nvb200_cache_attention_args *a, nvb2
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.status = a->status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (rows > kRows) {
+    const int rc = launch_cache_attention_wide(p, ct, a->head_dim, a->batch, a->num_splits, s);
+    if (rc != NVB200_ERR_UNSUPPORTED) return rc;
+  }
   switch (ct) {
     case kBf16: return launch_dim<kBf16>(p, a->head_dim, a->batch, a->num_splits, s);
     case kF16: return launch_dim<kF16>(p, a->head_dim, a->batch, a->num_splits, s);
