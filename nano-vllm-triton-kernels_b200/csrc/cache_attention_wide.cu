@@ -42,13 +42,13 @@ template <int CT, int D> struct Wide {
   static constexpr int NK = kQuant ? 1 : (D == 128 ? 2 : 4);
   static constexpr int NV = kQuant ? 1 : (D == 128 ? 3 : 4);
   static constexpr int NR = kQuant ? 2 : 0;
-  static constexpr int kSlots = kQuant ? 4 : 8;  // > NK + 2: a slot is rewritten only after its tile's softmax
+  static constexpr int kSlots = kQuant ? 4 : 8;  // >= NK + 3: a slot is rewritten only after its tile's softmax
   static constexpr int kOffK = kQBytes;
   static constexpr int kOffV = kOffK + NK * kOpBytes;
   static constexpr int kOffRaw = kOffV + NV * kOpBytes;
   static constexpr int kOffRawScale = kOffRaw + NR * 2 * kRawBytes;          // [NR][2][64] fp32: K scales, V scales
-  static constexpr int kOffScale = kOffRawScale + NR * 2 * kTileKeys * 4;  // [kSlots][3][64] fp32: K scales, V scales, log2 bounds
-  static constexpr int kSlotBytes = kQuant ? 3 * kTileKeys * 4 : 0;
+  static constexpr int kOffScale = kOffRawScale + NR * 2 * kTileKeys * 4;  // [kSlots] of [3][64] fp32 (K scales, V scales, log2 bounds) and 2 x the largest bound
+  static constexpr int kSlotBytes = kQuant ? 3 * kTileKeys * 4 + 16 : 0;
   static constexpr int kOffHdr = kOffScale + kSlots * kSlotBytes;
   static constexpr int kStride = D + 4;  // floats per merge record: o[D], m, l, M, flag
   static_assert(kOffHdr + 1024 <= kWideSmem, "a CTA's shared memory");
@@ -101,6 +101,19 @@ NVB200_DEVICE void tmem_st32(uint32_t taddr, const float (&v)[32]) {
                : "memory");
 }
 NVB200_DEVICE void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// max(a, b, c) as one instruction; a NaN operand is ignored, as by fmaxf.
+NVB200_DEVICE float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// (a, b) *= (c, d) in one packed instruction, each lane rounded as the scalar product.
+NVB200_DEVICE void mul2(float &a, float &b, float c, float d) {
+  const float2 r = f32x2_unpack(f32x2_mul(f32x2_pack(a, b), f32x2_pack(c, d)));
+  a = r.x, b = r.y;
+}
 
 NVB200_DEVICE void st_cluster_v4(uint32_t addr, float a, float b, float c, float d) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
@@ -375,30 +388,41 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
         }
         fence_proxy_async_smem();
       };
-      bool ok = true;
-      for (int i = 0; i < tiles; ++i) {
-        const int st = i % W::NR, slot = i % W::kSlots, sk = i % W::NK, sv = i % W::NV;
-        const int raw = W::kOffRaw + st * 2 * W::kRawBytes;
-        ok = wait(b_rfull + 8 * st, (i / W::NR) & 1) && wait(b_kempty + 8 * sk, ((i / W::NK) & 1) ^ 1);
-        if (!ok) break;
-        const uint32_t lo = ld_shared_u32(raw_live + 8 * st), hi = ld_shared_u32(raw_live + 8 * st + 4);
-        const unsigned long long live = static_cast<unsigned long long>(hi) << 32 | lo;
-        convert(raw, W::kOffK + sk * W::kOpBytes, live, false);
-        {
-          // The key's scales; zeros where it is none (its slot of the raw tile was not loaded).
-          const bool is = (live >> ct) & 1ull;
-          const float *rsc = reinterpret_cast<const float *>(smem + W::kOffRawScale + st * 2 * kTileKeys * 4);
-          const float ks = is ? rsc[ct] : 0.f, vs = is ? rsc[kTileKeys + ct] : 0.f;
-          float *sc = reinterpret_cast<float *>(smem + W::kOffScale + slot * W::kSlotBytes);
-          sc[ct] = ks, sc[kTileKeys + ct] = vs;
-          // Above log2 of the V scale: its exponent + 1.
-          sc[2 * kTileKeys + ct] = static_cast<float>(static_cast<int>(__float_as_uint(vs) >> 23 & 0xFFu) - 126);
-          if (ct == 0) st_shared_u32(live_slot + 8 * slot, lo), st_shared_u32(live_slot + 8 * slot + 4, hi);
+      auto live_of = [&](int st) {
+        return static_cast<unsigned long long>(ld_shared_u32(raw_live + 8 * st + 4)) << 32 | ld_shared_u32(raw_live + 8 * st);
+      };
+      auto convert_k = [&](int i) {
+        const int st = i % W::NR, slot = i % W::kSlots, sk = i % W::NK;
+        if (!wait(b_rfull + 8 * st, (i / W::NR) & 1) || !wait(b_kempty + 8 * sk, ((i / W::NK) & 1) ^ 1)) return false;
+        const unsigned long long live = live_of(st);
+        convert(W::kOffRaw + st * 2 * W::kRawBytes, W::kOffK + sk * W::kOpBytes, live, false);
+        // The key's scales; zeros where it is none (its slot of the raw tile was not loaded).
+        const bool is = (live >> ct) & 1ull;
+        const float *rsc = reinterpret_cast<const float *>(smem + W::kOffRawScale + st * 2 * kTileKeys * 4);
+        const float ks = is ? rsc[ct] : 0.f, vs = is ? rsc[kTileKeys + ct] : 0.f;
+        float *sc = reinterpret_cast<float *>(smem + W::kOffScale + slot * W::kSlotBytes);
+        sc[ct] = ks, sc[kTileKeys + ct] = vs;
+        // Above log2 of the V scale: its exponent + 1, and the largest of the warp's keys.
+        const int ve = static_cast<int>(__float_as_uint(vs) >> 23 & 0xFFu) - 126;
+        sc[2 * kTileKeys + ct] = static_cast<float>(ve);
+        const int top = __reduce_max_sync(0xffffffffu, ve);
+        if (lane == 0) sc[3 * kTileKeys + (warp - 6)] = static_cast<float>(top);
+        if (ct == 0) {
+          st_shared_u32(live_slot + 8 * slot, static_cast<uint32_t>(live));
+          st_shared_u32(live_slot + 8 * slot + 4, static_cast<uint32_t>(live >> 32));
         }
         arrive(b_kfull + 8 * sk);
-        ok = wait(b_vempty + 8 * sv, ((i / W::NV) & 1) ^ 1);
+        return true;
+      };
+      // K of the next tile goes before V of this one: its product is wanted first, and V's buffer is only free once P V of
+      // the tile before is done.
+      bool ok = tiles == 0 || convert_k(0);
+      for (int i = 0; i < tiles && ok; ++i) {
+        if (i + 1 < tiles) ok = convert_k(i + 1);
+        const int st = i % W::NR, sv = i % W::NV;
+        ok = ok && wait(b_vempty + 8 * sv, ((i / W::NV) & 1) ^ 1);
         if (!ok) break;
-        convert(raw + W::kRawBytes, W::kOffV + sv * W::kOpBytes, live,
+        convert(W::kOffRaw + st * 2 * W::kRawBytes + W::kRawBytes, W::kOffV + sv * W::kOpBytes, live_of(st),
                 hides && js + (i + 1) * kTileKeys > open);
         arrive(b_vfull + 8 * sv);
         arrive(b_rempty + 8 * st);
@@ -536,16 +560,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
         }
       }
       if (warp_live) {
-        float x[kTileKeys];  // scores before the row's factor rs > 0
-        tmem_ld64(s_addr, x);
         const float4 *sc = reinterpret_cast<const float4 *>(smem + W::kOffScale + slot * W::kSlotBytes);
-        if constexpr (W::kQuant) {
-#pragma unroll
-          for (int c = 0; c < kTileKeys; c += 4) {
-            const float4 k4 = sc[c / 4];
-            x[c] *= k4.x, x[c + 1] *= k4.y, x[c + 2] *= k4.z, x[c + 3] *= k4.w;
-          }
-        }
         uint32_t see_lo = 0xFFFFFFFFu, see_hi = 0xFFFFFFFFu;
         if (edge) {
           unsigned long long see = ~0ull;
@@ -565,20 +580,59 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
           }
           if (qi < 0) see = 0ull;
           see_lo = lo & static_cast<uint32_t>(see), see_hi = hi & static_cast<uint32_t>(see >> 32);
-#pragma unroll
-          for (int c = 0; c < kTileKeys; ++c)
-            if (!((c < 32 ? see_lo >> c : see_hi >> (c - 32)) & 1u)) x[c] = -INFINITY;
         }
-        float mx = x[0], mx1 = x[1], Mt = M;
+        // Scores of columns c0 .. c0 + CW before the row's factor rs > 0. 8-bit caches read S twice, 32 columns at a time
+        // (for the maximum, then for the weights): a tile's 64 scores beside three numbers per key do not fit the
+        // registers of a thread, and what is spilled goes to the L2, the L1 being all shared memory here.
+        constexpr int CW = W::kQuant ? 32 : 64;
+        float x[CW];
+        auto scores = [&](int c0) {
+          if constexpr (W::kQuant) {
+            tmem_ld32(s_addr + c0, x);
 #pragma unroll
-        for (int c = 2; c < kTileKeys; c += 2) mx = fmaxf(mx, x[c]), mx1 = fmaxf(mx1, x[c + 1]);
-        const float mt = fmaxf(m, fmaxf(mx, mx1) * rs);
+            for (int c = 0; c < CW; c += 4) {
+              const float4 k4 = sc[(c0 + c) / 4];
+              mul2(x[c], x[c + 1], k4.x, k4.y);
+              mul2(x[c + 2], x[c + 3], k4.z, k4.w);
+            }
+          } else {
+            tmem_ld64(s_addr, x);
+          }
+          if (edge) {
+#pragma unroll
+            for (int c = 0; c < CW; ++c) {
+              const uint32_t see = CW == 64 ? (c < 32 ? see_lo : see_hi) : (c0 ? see_hi : see_lo);
+              if (!((see >> (c & 31)) & 1u)) x[c] = -INFINITY;
+            }
+          }
+        };
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c0 = 0; c0 < kTileKeys; c0 += CW) {
+          scores(c0);
+          float mx = fmax3(top, x[0], x[1]), mx1 = fmaxf(x[2], x[3]);
+#pragma unroll
+          for (int c = 4; c < CW; c += 4) mx = fmax3(mx, x[c], x[c + 1]), mx1 = fmax3(mx1, x[c + 2], x[c + 3]);
+          top = fmaxf(mx, mx1);
+        }
+        top *= rs;  // the tile's largest score
+        const float mt = fmaxf(m, top);
+        // The weights' reference: while the tile's largest score and its largest V scale together stay below M + 8 no
+        // weight can exceed it; only otherwise is the row's own maximum taken.
+        float Mt = M;
         if constexpr (W::kQuant) {
+          const float2 bound = *reinterpret_cast<const float2 *>(sc + 3 * kTileKeys / 4);
+          if (__any_sync(0xffffffffu, top + fmaxf(bound.x, bound.y) > M + 8.f || M == -INFINITY)) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < kTileKeys; c0 += CW) {
+              scores(c0);
 #pragma unroll
-          for (int c = 0; c < kTileKeys; c += 4) {
-            const float4 e4 = sc[(2 * kTileKeys + c) / 4];
-            Mt = fmaxf(Mt, fmaxf(fmaf(x[c], rs, e4.x), fmaf(x[c + 1], rs, e4.y)));
-            Mt = fmaxf(Mt, fmaxf(fmaf(x[c + 2], rs, e4.z), fmaf(x[c + 3], rs, e4.w)));
+              for (int c = 0; c < CW; c += 4) {
+                const float4 e4 = sc[(2 * kTileKeys + c0 + c) / 4];
+                Mt = fmax3(Mt, fmaf(x[c], rs, e4.x), fmaf(x[c + 1], rs, e4.y));
+                Mt = fmax3(Mt, fmaf(x[c + 2], rs, e4.z), fmaf(x[c + 3], rs, e4.w));
+              }
+            }
           }
         }
         // The references move only when they are exceeded by 8 (a factor 256), or are not set yet.
@@ -605,35 +659,38 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
         }
         const float mu = m == -INFINITY ? 0.f : m;
         const float cw = W::kQuant ? ex2_approx_ftz(mu - (M == -INFINITY ? 0.f : M)) : 1.f;
-        float sum0 = 0.f, sum1 = 0.f;
+        uint64_t sum0 = 0, sum1 = 0;  // pairs of fp32
+#pragma unroll 1
+        for (int c0 = 0; c0 < kTileKeys; c0 += CW) {
+          if constexpr (W::kQuant) scores(c0);
 #pragma unroll
-        for (int c0 = 0; c0 < kTileKeys; c0 += 32) {
-          uint32_t pk[16];
+          for (int h0 = 0; h0 < CW; h0 += 32) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            float w[4];
-            float4 v4 = make_float4(1.f, 1.f, 1.f, 1.f);
-            if constexpr (W::kQuant) v4 = sc[(kTileKeys + c0 + c) / 4];
-            const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+            for (int c = 0; c < 32; c += 4) {
+              float w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              w[e] = ex2_approx_ftz(fmaf(x[c0 + c + e], rs, -mu));
-              if (e & 1) sum1 += w[e];
-              else sum0 += w[e];
-              if constexpr (W::kQuant) w[e] = w[e] * vv[e] * cw;
+              for (int e = 0; e < 4; ++e) w[e] = ex2_approx_ftz(fmaf(x[h0 + c + e], rs, -mu));
+              sum0 = f32x2_add(sum0, f32x2_pack(w[0], w[1])), sum1 = f32x2_add(sum1, f32x2_pack(w[2], w[3]));
+              if constexpr (W::kQuant) {
+                const float4 v4 = sc[(kTileKeys + c0 + c) / 4];
+                mul2(w[0], w[1], v4.x, v4.y), mul2(w[0], w[1], cw, cw);
+                mul2(w[2], w[3], v4.z, v4.w), mul2(w[2], w[3], cw, cw);
+              }
+              pk[c / 2] = C::kBf16Mma ? pack_bf16x2(w[0], w[1]) : pack_f16x2(w[0], w[1]);
+              pk[c / 2 + 1] = C::kBf16Mma ? pack_bf16x2(w[2], w[3]) : pack_f16x2(w[2], w[3]);
             }
-            pk[c / 2] = C::kBf16Mma ? pack_bf16x2(w[0], w[1]) : pack_f16x2(w[0], w[1]);
-            pk[c / 2 + 1] = C::kBf16Mma ? pack_bf16x2(w[2], w[3]) : pack_f16x2(w[2], w[3]);
-          }
-          if (W::kQuant && edge) {  // 0 times a NaN row scale
-            const uint32_t see = c0 ? see_hi : see_lo;
+            if (W::kQuant && edge) {  // 0 times a NaN row scale
+              const uint32_t see = c0 ? see_hi : see_lo;
 #pragma unroll
-            for (int c = 0; c < 16; ++c)
-              pk[c] &= ((see >> (2 * c)) & 1u ? 0xFFFFu : 0u) | ((see >> (2 * c + 1)) & 1u ? 0xFFFF0000u : 0u);
+              for (int c = 0; c < 16; ++c)
+                pk[c] &= ((see >> (2 * c)) & 1u ? 0xFFFFu : 0u) | ((see >> (2 * c + 1)) & 1u ? 0xFFFF0000u : 0u);
+            }
+            tmem_st16(s_addr + (c0 + h0) / 2, pk);  // over scores that have been read
           }
-          tmem_st16(s_addr + c0 / 2, pk);
         }
-        l += sum0 + sum1;
+        const float2 sum = f32x2_unpack(f32x2_add(sum0, sum1));
+        l += sum.x + sum.y;
         tmem_st_wait();
       }
       tc_fence_before();
