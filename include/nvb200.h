@@ -396,7 +396,9 @@ NVB200_API int nvb200_load_kvcache_quant(void *key, void *value, const nvb200_qu
  *   q: [batch, n, num_q_heads, head_dim] with the given strides, unit last stride; dtype bf16 or fp16.
  *   cache_dtype: = dtype (16-bit cache, strides as given, unit last stride), or NVB200_E4M3 / NVB200_I8 with k_scale and
  *     v_scale contiguous [num_blocks, num_kv_heads, block_size] (see nvb200_quant_cache).
- *   block_table, seqlens, num_splits, softmax_scale, status: as for nvb200_paged_decode_attention. Keys whose block-table
+ *   num_splits: 0: chosen from the sizes (even shares of all sequences' keys over the GPU, or a cluster of CTAs per
+ *     sequence); 1..8: that many CTAs (a thread-block cluster) share each sequence's keys.
+ *   block_table, seqlens, softmax_scale, status: as for nvb200_paged_decode_attention. Keys whose block-table
  *     entry lies outside [0, num_blocks) are seen by no row; they, lengths beyond max_blocks_per_seq * block_size
  *     and draft_lens outside [0, n] (both clamped) set NVB200_STATUS_BAD_SLOT.
  *   out: [batch, n, num_q_heads, head_dim] contiguous, dtype, written.
@@ -439,7 +441,13 @@ typedef struct nvb200_cache_attention_args {
   int32_t *status;
 } nvb200_cache_attention_args;
 
-NVB200_API int nvb200_cache_attention(const nvb200_cache_attention_args *args, nvb200_stream_t stream);
+/* workspace: device memory of nvb200_cache_attention_workspace_size(args) bytes, 16-byte aligned, of any content; calls that
+ * may run at the same time need separate ones. 0 bytes (and NULL) where the call needs none; NULL elsewhere runs a form
+ * that needs none, slower for ragged batches and for many query rows. The size depends on args' sizes alone (-1: args that
+ * the call refuses). Returns NVB200_ERR_ARG for a workspace that is too small. */
+NVB200_API int64_t nvb200_cache_attention_workspace_size(const nvb200_cache_attention_args *args);
+NVB200_API int nvb200_cache_attention(const nvb200_cache_attention_args *args, void *workspace, int64_t workspace_bytes,
+                                      nvb200_stream_t stream);
 
 #ifdef __cplusplus
 }

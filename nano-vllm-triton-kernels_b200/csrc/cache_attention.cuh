@@ -27,7 +27,10 @@ struct CacheAttnParams {
   const uint8_t *mask;        // [batch, n, n] bytes, NULL: chain (causal) or no mask
   int64_t mask_batch_stride, mask_row_stride;
   void *out;                  // [batch, n, hq, D] contiguous
-  int n, hq, hkv, group, block_size, bs_shift, max_pages, rows, causal, splits;
+  int n, hq, hkv, group, block_size, bs_shift, max_pages, rows, causal;
+  int batch;
+  int splits;      // CTAs of a cluster sharing the keys of a sequence (cluster form)
+  float *records;  // workspace of the even-share form: [2 * grid] records of [block_rows][D + 4] floats
   int q_is_f16;
   float scale_log2;
   int32_t *status;
@@ -96,6 +99,144 @@ template <int CT> NVB200_DEVICE uint32_t nonfinite_bits(uint32_t w) {
   return __vcmpeq2(w & kExp, kExp);
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Even shares of a batch whose lengths the host does not know. The work of a call is a sequence of key tiles, ordered by
+// sequence, then unit (KV head, block of query rows), then tile; CTA c of G takes tiles [c T / G, (c + 1) T / G). A
+// segment is the part of one unit in one CTA's range. A unit inside one range is finished there; one that a range's end
+// cuts leaves a record per CTA in the workspace (only the first and the last segment of a range can be cut: two slots per
+// CTA), which a second kernel merges in the order of the CTAs. No CTA waits for another, and nothing outlives the call.
+
+struct SeqInfo {
+  int L, drafts;  // keys, and how many of them (the last) are the new tokens
+  int tiles;      // of keys
+  int blocks;     // of query rows that hold new tokens
+};
+
+// `report`: flag lengths that had to be clamped.
+NVB200_DEVICE SeqInfo seq_info(const CacheAttnParams &p, int b, int tile_keys, int block_rows, bool report = false) {
+  SeqInfo s;
+  s.L = __ldg(p.seqlens + b);
+  s.drafts = p.draft_lens ? __ldg(p.draft_lens + b) : p.n;
+  const int64_t cap = static_cast<int64_t>(p.max_pages) * p.block_size;
+  if (s.L < 0 || s.L > cap || s.drafts < 0 || s.drafts > p.n) {
+    if (report) set_status(p.status, NVB200_STATUS_BAD_SLOT);
+    s.L = s.L < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(s.L), cap));
+    s.drafts = max(0, min(s.drafts, p.n));
+  }
+  s.tiles = (s.L + tile_keys - 1) / tile_keys;
+  s.blocks = s.L > 0 ? (s.drafts * p.group + block_rows - 1) / block_rows : 0;
+  if (s.blocks == 0) s.tiles = 0;
+  return s;
+}
+
+// Tiles of sequence b over all its units.
+NVB200_DEVICE int seq_work(const CacheAttnParams &p, int b, int tile_keys, int block_rows) {
+  const SeqInfo s = seq_info(p, b, tile_keys, block_rows);
+  return s.tiles * s.blocks * p.hkv;
+}
+
+// First tile of CTA c, and the CTA that has tile u, of T tiles over G <= T CTAs.
+NVB200_DEVICE int range_start(int64_t c, int64_t T, int64_t G) { return static_cast<int>(c * T / G); }
+NVB200_DEVICE int range_owner(int64_t u, int64_t T, int64_t G) { return static_cast<int>(((u + 1) * G - 1) / T); }
+// Record slot of CTA c for the unit that starts at tile unit_u.
+NVB200_DEVICE int record_slot(int c, int unit_u, int64_t T, int64_t G) {
+  return 2 * c + (unit_u <= range_start(c, T, G) ? 0 : 1);
+}
+
+// The part of one unit in a CTA's range. The same in every thread that walks it.
+struct Segment {
+  int u;       // global index of its first tile
+  int unit_u;  // ... of the unit's first tile
+  int unit;    // h * blocks + block
+  int t0, n;   // its tiles within the unit; n = 0: the range is exhausted
+  int b;
+  SeqInfo s;
+};
+
+// The segment that holds tile u < T, ending at u1 or with its unit. Warp-wide.
+NVB200_DEVICE Segment find_segment(const CacheAttnParams &p, int u, int u1, int tile_keys, int block_rows) {
+  const int lane = threadIdx.x & 31;
+  Segment g;
+  g.u = u;
+  int before = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int b = b0 + lane;
+    int x = b < p.batch ? seq_work(p, b, tile_keys, block_rows) : 0;
+    const int mine = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + x > u);
+    if (hit != 0 || b0 + 32 >= p.batch) {
+      const int at = hit ? __ffs(hit) - 1 : 31;
+      g.b = b0 + at;
+      before += __shfl_sync(0xffffffffu, x - mine, at);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, x, 31);
+  }
+  g.s = seq_info(p, g.b, tile_keys, block_rows);
+  const int in = u - before;
+  g.unit = in / g.s.tiles;
+  g.t0 = in - g.unit * g.s.tiles;
+  g.unit_u = u - g.t0;
+  g.n = min(g.s.tiles - g.t0, u1 - u);
+  return g;
+}
+
+// Moves on to the next unit of the range [., u1).
+NVB200_DEVICE void next_segment(Segment &g, const CacheAttnParams &p, int u1, int tile_keys, int block_rows) {
+  g.u += g.n;
+  if (g.u >= u1) {
+    g.n = 0;
+    return;
+  }
+  if (++g.unit == g.s.blocks * p.hkv) {
+    g.unit = 0;
+    do {
+      g.s = seq_info(p, ++g.b, tile_keys, block_rows);
+    } while (g.s.tiles == 0);  // g.u < u1 <= T: there is one with tiles
+  }
+  g.unit_u = g.u, g.t0 = 0;
+  g.n = min(g.s.tiles, u1 - g.u);
+}
+
+// T, by a whole warp.
+NVB200_DEVICE int total_work(const CacheAttnParams &p, int tile_keys, int block_rows) {
+  int x = 0;
+  for (int b = threadIdx.x & 31; b < p.batch; b += 32) x += seq_work(p, b, tile_keys, block_rows);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// CTAs that get work: fewer than are launched when the tiles are few.
+NVB200_DEVICE int active_ctas(int T, int grid, int min_tiles) { return max(1, min(grid, T / min_tiles)); }
+
+// Rows of the output that no unit covers (tokens behind draft_lens[b] beyond the last block, sequences without keys):
+// zeros, CTA c of `grid` taking every grid-th sequence. Also reports clamped lengths.
+NVB200_DEVICE void zero_uncovered_rows(const CacheAttnParams &p, int head_dim, int tile_keys, int block_rows, int c, int grid,
+                                       int tid, int threads) {
+  for (int b = c; b < p.batch; b += grid) {
+    const SeqInfo s = seq_info(p, b, tile_keys, block_rows, tid == 0);
+    const int from = min(s.blocks * block_rows, p.n * p.group);
+    // Row r of KV head h is token r / group, head h * group + r % group. 16-byte pieces where `out` allows.
+    const int rows = p.n * p.group - from;
+    const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+    const int pieces = wide ? head_dim / 8 : head_dim;
+    for (int h = 0; h < p.hkv; ++h) {
+      for (int e = tid; e < rows * pieces; e += threads) {
+        const int r = from + e / pieces, d = e % pieces, qi = r / p.group;
+        const int64_t row = ((static_cast<int64_t>(b) * p.n + qi) * p.hq + h * p.group + r - qi * p.group) * head_dim;
+        if (wide) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + row + 8 * d) = make_uint4(0u, 0u, 0u, 0u);
+        else static_cast<uint16_t *>(p.out)[row + d] = 0;
+      }
+    }
+  }
+}
+
 NVB200_DEVICE int page_of(const CacheAttnParams &p, int j) {
   return p.bs_shift >= 0 ? j >> p.bs_shift : j / p.block_size;
 }
@@ -129,7 +270,12 @@ NVB200_DEVICE float add_nonfinite(const CacheAttnParams &p, const int32_t *bt, i
 
 // The wide kernel (cache_attention_wide.cu). NVB200_ERR_UNSUPPORTED where it does not take the call (pages whose size is
 // not a multiple of 8 tokens, cache strides that no tensor map describes).
-int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, int batch, int num_splits,
-                                cudaStream_t stream);
+bool wide_takes(const CacheAttnParams &p);
+int64_t wide_workspace_bytes(const CacheAttnParams &p, int head_dim);
+int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, cudaStream_t stream);
+
+// Merges the records of the units that range ends cut, after a grid of `grid` CTAs.
+int launch_cache_attention_merge(const CacheAttnParams &p, int ct, int head_dim, int tile_keys, int block_rows,
+                                 int min_tiles, int grid, cudaStream_t stream);
 
 }  // namespace nvb200

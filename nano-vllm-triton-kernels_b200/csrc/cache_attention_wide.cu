@@ -2,17 +2,17 @@
 // per CTA, on the 5th-generation tensor cores. For trees and chains whose tokens x group fill more than the 16 rows of
 // the warp-level kernel, which would read and convert the keys once per 16 rows.
 //
-// A CTA takes 128 rows (token i, head of the group) of one (sequence, KV head) and a share of the keys, in tiles of 64:
+// A CTA takes 128 rows (token i, head of the group) of one (sequence, KV head) and a run of its keys, in tiles of 64:
 //   * warp 4, the producer: K and V tiles by TMA from the paged cache (one box per page run), into a ring;
-//   * 8-bit caches: warps 6 and 7 convert the landed codes to fp16 operand tiles (exact), and bring the row scales;
+//   * 8-bit caches: warps 6 to 9 convert the landed codes to fp16 operand tiles (exact), and bring the row scales;
 //   * warp 5, one lane: S = Q K^T (128 x 64, fp32, one of two TMEM buffers), later O += P V (128 x D, fp32, TMEM), with
 //     P read from TMEM, where it overwrites its S;
 //   * warps 0-3, one thread per row: the running softmax. The maximum that weights refer to moves only when a row exceeds
 //     it by 2^8 (weights stay below 2^9, in range for fp16), so O is rarely rescaled; the sums are fp32.
-// Two CTAs share an SM (113 KB of shared memory and 256 TMEM columns each): the one computes while the other waits. CTAs
-// of a cluster split the keys and merge through distributed shared memory, each finishing every splits-th row.
-// Waits are bounded; a CTA that gives up sets NVB200_STATUS_WAIT_TIMEOUT, lets its copies land and still takes the cluster
-// barriers.
+// Two CTAs share an SM (113 KB of shared memory and 256 TMEM columns each): the one computes while the other waits. The
+// grid is what the GPU holds at once, and each CTA takes an even share of the batch's tiles (cache_attention.cuh); the
+// roles walk the CTA's segments independently, so the loads of a segment start while the one before is finished.
+// Waits are bounded; a CTA that gives up sets NVB200_STATUS_WAIT_TIMEOUT and lets its copies land.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -27,14 +27,16 @@ constexpr int kTileKeys = 64;
 constexpr int kTileRows = 128;
 constexpr int kTmemCols = 256;  // S: 2 x 64, O: up to 128
 constexpr int kColO = 128;
+constexpr int kPrefetch = 5;  // tiles ahead of the one being loaded that are brought into the L2
+constexpr int kMinTiles = 4;  // of a CTA, where there are too few for all
 // Shared memory of a CTA: exactly two fit on an SM (228 KB, 1 KB of it reserved per CTA). Nothing that holds TMEM fits
 // beside two, so a CTA never waits for TMEM that a CTA of another kernel holds.
 constexpr int kWideSmem = 113 * 1024;
 
 template <int CT, int D> struct Wide {
   static constexpr bool kQuant = CacheType<CT>::kQuant;
-  static constexpr int kThreads = kQuant ? 256 : 192;
-  static constexpr int kConvWarps = 2;
+  static constexpr int kThreads = kQuant ? 320 : 192;
+  static constexpr int kConvWarps = 4;  // one per scheduler
   static constexpr int kQBytes = kTileRows * D * 2;
   static constexpr int kOpBytes = kTileKeys * D * 2;  // a K or V operand tile
   static constexpr int kRawBytes = kTileKeys * D;     // the same as codes
@@ -47,12 +49,10 @@ template <int CT, int D> struct Wide {
   static constexpr int kOffV = kOffK + NK * kOpBytes;
   static constexpr int kOffRaw = kOffV + NV * kOpBytes;
   static constexpr int kOffRawScale = kOffRaw + NR * 2 * kRawBytes;          // [NR][2][64] fp32: K scales, V scales
-  static constexpr int kOffScale = kOffRawScale + NR * 2 * kTileKeys * 4;  // [kSlots] of [3][64] fp32 (K scales, V scales, log2 bounds) and 2 x the largest bound
+  static constexpr int kOffScale = kOffRawScale + NR * 2 * kTileKeys * 4;  // [kSlots] of [3][64] fp32 (K scales, V scales, log2 bounds), 2 x largest and 2 x smallest bound
   static constexpr int kSlotBytes = kQuant ? 3 * kTileKeys * 4 + 16 : 0;
   static constexpr int kOffHdr = kOffScale + kSlots * kSlotBytes;
-  static constexpr int kStride = D + 4;  // floats per merge record: o[D], m, l, M, flag
   static_assert(kOffHdr + 1024 <= kWideSmem, "a CTA's shared memory");
-  static_assert((kTileRows + kMaxSplits) * kStride * 4 <= kOffHdr, "merge records fit below the barriers");
 };
 
 struct WideMaps {
@@ -70,6 +70,13 @@ NVB200_DEVICE void tma_load_4d(uint32_t dst, const CUtensorMap *map, int c0, int
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
       "[%6];" ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
+}
+
+// Brings a box into the L2.
+NVB200_DEVICE void tma_prefetch_4d(const CUtensorMap *map, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c0), "r"(c1),
+               "r"(c2), "r"(c3)
+               : "memory");
 }
 
 // D[tmem] (+)= A[tmem] B[shared], 16-bit operands.
@@ -115,15 +122,13 @@ NVB200_DEVICE void mul2(float &a, float &b, float c, float d) {
   a = r.x, b = r.y;
 }
 
-NVB200_DEVICE void st_cluster_v4(uint32_t addr, float a, float b, float c, float d) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
-               : "memory");
-}
-
 // Swizzled position of 16-byte chunk c (0-7) of 128-byte row r in a tile of such rows.
 NVB200_DEVICE uint32_t swz128(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
 
-template <int CT, int D>
+// REP = 2 (at most 64 rows): every row twice in the 128 lanes of a tile, lane r taking keys 0-31 of each tile and lane 64 +
+// r keys 32-63, as if they were two shares of the keys; the tile's products cost what they cost for 128 rows, but a softmax
+// thread has half the work.
+template <int CT, int D, int REP>
 __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
     cache_attention_wide_kernel(const __grid_constant__ WideParams wp, const __grid_constant__ WideMaps maps) {
   using W = Wide<CT, D>;
@@ -133,16 +138,20 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
   extern __shared__ __align__(1024) uint8_t smem[];
   const CacheAttnParams &p = wp.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int row_tiles = (p.rows + kTileRows - 1) / kTileRows;
-  const int h = blockIdx.y / row_tiles, row0 = (blockIdx.y - h * row_tiles) * kTileRows;
-  const int b = blockIdx.z;
-  const int nrows = min(kTileRows, p.rows - row0);
-  const uint32_t rank = p.splits > 1 ? cta_rank_in_cluster() : 0u;
+  constexpr int kUnitRows = kTileRows / REP;  // rows of a unit
   const uint32_t base = smem_addr(smem);
+  const int T = total_work(p, kTileKeys, kUnitRows);  // by every warp
+  const int G = active_ctas(T, gridDim.x, kMinTiles);
+  zero_uncovered_rows(p, D, kTileKeys, kUnitRows, blockIdx.x, gridDim.x, tid, W::kThreads);
+  if (T == 0 || static_cast<int>(blockIdx.x) >= G) return;
+  const int u0 = range_start(blockIdx.x, T, G), u1 = range_start(blockIdx.x + 1, T, G);
+  Segment seg = find_segment(p, u0, u1, kTileKeys, kUnitRows);
+  auto next = [&]() { next_segment(seg, p, u1, kTileKeys, kUnitRows); };
 
   const uint32_t hdr = base + W::kOffHdr;
   const uint32_t b_kfull = hdr, b_kempty = hdr + 32, b_vfull = hdr + 64, b_vempty = hdr + 96;  // up to 4 each
-  const uint32_t b_sfull = hdr + 128, b_pready = hdr + 144, b_pv = hdr + 160, b_q = hdr + 168;
+  const uint32_t b_sfull = hdr + 128, b_pready = hdr + 144, b_q = hdr + 168, b_meet = hdr + 176;
+  const uint32_t b_pv = hdr + 184;  // 2, like b_sfull and b_pready by tile parity: the softmax may be two P V ahead of one
   const uint32_t b_rfull = hdr + 240, b_rempty = hdr + 272;              // up to 4 each
   const uint32_t live_slot = hdr + 304, raw_live = hdr + 368;            // 64-bit words: up to 8, up to 4
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + W::kOffHdr + 400);
@@ -151,9 +160,8 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
   if (tid == 0) {
     for (int i = 0; i < W::NK; ++i) mbar_init(b_kfull + 8 * i, W::kQuant ? W::kConvWarps : 1), mbar_init(b_kempty + 8 * i, 1);
     for (int i = 0; i < W::NV; ++i) mbar_init(b_vfull + 8 * i, W::kQuant ? W::kConvWarps : 1), mbar_init(b_vempty + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(b_sfull + 8 * i, 2), mbar_init(b_pready + 8 * i, 4);
-    mbar_init(b_pv, 1);
-    mbar_init(b_q, 4);
+    for (int i = 0; i < 2; ++i) mbar_init(b_sfull + 8 * i, 2), mbar_init(b_pready + 8 * i, 4), mbar_init(b_pv + 8 * i, 1);
+    mbar_init(b_q, 4), mbar_init(b_meet, 4);
     for (int i = 0; i < W::NR; ++i) mbar_init(b_rfull + 8 * i, 1), mbar_init(b_rempty + 8 * i, W::kConvWarps);
     st_shared_u32(failed, 0u), st_shared_u32(dirty, 0u);
     fence_mbar_init();
@@ -164,27 +172,6 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-
-  // Keys [0, L), of which the last `drafts` are the new tokens.
-  int L = p.seqlens[b];
-  int drafts = p.draft_lens ? p.draft_lens[b] : p.n;
-  const int64_t cap = static_cast<int64_t>(p.max_pages) * p.block_size;
-  if (L < 0 || L > cap || drafts < 0 || drafts > p.n) {
-    if (tid == 0 && rank == 0) set_status(p.status, NVB200_STATUS_BAD_SLOT);
-    L = L < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(L), cap));
-    drafts = max(0, min(drafts, p.n));
-  }
-  const int ctx = L - drafts;
-  const bool masked = p.mask != nullptr || p.causal;
-  const int open = masked ? max(ctx, 0) : L;      // every row sees the keys below this
-  const bool any_row = row0 / p.group < drafts;   // else all rows of this CTA are padding
-  const int per = any_row ? ((L + p.splits - 1) / p.splits + kTileKeys - 1) / kTileKeys * kTileKeys : 0;
-  const int js = static_cast<int>(min(static_cast<int64_t>(L), static_cast<int64_t>(rank) * per));
-  const int je = any_row ? min(L - js, per) + js : js;
-  const int tiles = (je - js + kTileKeys - 1) / kTileKeys;
-  const int32_t *bt = p.block_table ? p.block_table + b * p.bt_stride : nullptr;
-  // A tile in which a row may not see a key that others see, so that V must be finite (see add_nonfinite).
-  const bool hides = p.mask ? drafts > 0 : (p.causal && drafts > 1);
 
   auto give_up = [&]() {
     set_status(p.status, NVB200_STATUS_WAIT_TIMEOUT);
@@ -205,27 +192,54 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
     if (lane == 0) mbar_arrive(bar);
   };
 
-  // Merge state of this thread's row (softmax warps).
-  float m = -INFINITY, l = 0.f, M = -INFINITY;
+  const bool masked = p.mask != nullptr || p.causal;
+  // Of the current segment: first tile's first key, end of its keys; keys before the new tokens; every row sees the keys
+  // below `open`; whether a row may not see a key that others see (V must then be finite: see add_nonfinite).
+  auto first_key = [&]() { return seg.t0 * kTileKeys; };
+  auto end_key = [&]() { return min(static_cast<int64_t>(seg.s.L), static_cast<int64_t>(seg.t0 + seg.n) * kTileKeys); };
+  auto context = [&]() { return seg.s.L - seg.s.drafts; };
+  auto open_below = [&]() { return masked ? max(context(), 0) : seg.s.L; };
+  auto hides_keys = [&]() { return p.mask ? seg.s.drafts > 0 : (p.causal && seg.s.drafts > 1); };
+  auto table_of = [&]() { return p.block_table ? p.block_table + seg.b * p.bt_stride : nullptr; };
 
   if (warp == 4) {
     // ---------------------------------------------------------------- producer: lane r has box r of every tile
     const int R = wp.box_rows, boxes = kTileKeys / R;
     const uint32_t row_bytes = D * C::kBytes;
-    auto block_at = [&](int i) {
-      const int j = js + i * kTileKeys + lane * R;
+    int i = 0;  // tile of the CTA
+    bool go = true;
+    for (; seg.n > 0 && go; next()) {
+    const int32_t *bt = table_of();
+    const int b = seg.b, h = seg.unit / seg.s.blocks, js = first_key(), je = static_cast<int>(end_key());
+    auto block_at = [&](int t) {
+      const int j = js + t * kTileKeys + lane * R;
       return lane < boxes && j < je ? (bt ? __ldg(bt + page_of(p, j)) : b) : -1;
     };
-    int blk = tiles > 0 ? block_at(0) : -1;
-    int issued = 0;
-    for (int i = 0; i < tiles; ++i) {
-      const int j = js + i * kTileKeys + lane * R;
+    auto prefetch = [&](int t, int block) {
+      if (block < 0 || block >= p.num_blocks) return;
+      const int j = js + t * kTileKeys + lane * R, tok = j - page_of(p, j) * p.block_size;
+#pragma unroll
+      for (int u = 0; u < (W::kQuant ? 1 : D / 64); ++u) {
+        tma_prefetch_4d(&maps.k, 64 * u, tok, h, block);
+        tma_prefetch_4d(&maps.v, 64 * u, tok, h, block);
+      }
+    };
+    int blk = block_at(0), far = -1;
+    for (int t = 0; t < seg.n; ++t, ++i) {
+      const int j = js + t * kTileKeys + lane * R;
       const bool mine = lane < boxes && j < je;
       const bool ok = mine && blk >= 0 && blk < p.num_blocks;
       if (mine && !ok) set_status(p.status, NVB200_STATUS_BAD_SLOT);
       const int here = blk, page = mine ? page_of(p, j) : 0;
       const int tok = j - page * p.block_size;
-      if (i + 1 < tiles) blk = block_at(i + 1);
+      if (t + 1 < seg.n) blk = block_at(t + 1);
+      // The ring holds two or three tiles, less than HBM's latency wants: tiles further ahead start their way into the L2.
+      if (t == 0) {
+        for (int a = 1; a <= kPrefetch; ++a) prefetch(a, a < seg.n ? block_at(a) : -1);
+      } else {
+        prefetch(t + kPrefetch, far);
+      }
+      far = t + 1 + kPrefetch < seg.n ? block_at(t + 1 + kPrefetch) : -1;
       // Bit k: key k of the tile exists and its page can be followed.
       unsigned long long bits = 0;
       if (ok) {
@@ -235,7 +249,6 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
       const uint32_t lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(bits));
       const uint32_t hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(bits >> 32));
       const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, ok)) * R * row_bytes;
-      bool go;
       if constexpr (W::kQuant) {
         const int st = i % W::NR;
         go = wait(b_rempty + 8 * st, ((i / W::NR) & 1) ^ 1);
@@ -283,9 +296,10 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
                         h, here, b_vfull + 8 * sv);
         }
       }
-      ++issued;
     }
-    if (issued < tiles) {
+    }
+    const int issued = i;
+    if (!go) {
       // Gave up: let the copies in flight land before the shared memory is released.
       if (lane == 0) {
         give_up();
@@ -326,34 +340,39 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
       __syncwarp();
       return true;
     };
-    bool ok = tiles == 0 || (wait(b_q, 0) && qk(0));
-    for (int i = 0; i < tiles && ok; ++i) {
-      // S of the next tile before this tile's P V: the softmax has it while P V runs. Its buffer's P was consumed by
-      // the P V of tile i - 1, issued before it.
-      if (i + 1 < tiles) ok = qk(i + 1);
-      const int st = i % W::NV;
-      ok = ok && wait(b_pready + 8 * (i & 1), (i >> 1) & 1) && wait(b_vfull + 8 * st, (i / W::NV) & 1);
-      if (!ok) break;
-      tc_fence_after();
-      const uint64_t bd = smem_desc(base + W::kOffV + st * W::kOpBytes, kTileKeys * 128, 1024, 2);
-      const uint32_t pa = td + (i & 1) * kTileKeys;
-      if (lane == 0) {
+    bool ok = true;
+    int i = 0;  // tile of the CTA
+    for (int q = 0; seg.n > 0 && ok; next(), ++q) {
+      // The segment's query rows are in place, which also says that the softmax is done with O of the segment before.
+      ok = wait(b_q, q & 1) && qk(i);
+      for (int t = 0; t < seg.n && ok; ++t, ++i) {
+        // S of the next tile before this tile's P V: the softmax has it while P V runs. Its buffer's P was consumed by
+        // the P V of tile i - 1, issued before it.
+        if (t + 1 < seg.n) ok = qk(i + 1);
+        const int st = i % W::NV;
+        ok = ok && wait(b_pready + 8 * (i & 1), (i >> 1) & 1) && wait(b_vfull + 8 * st, (i / W::NV) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t bd = smem_desc(base + W::kOffV + st * W::kOpBytes, kTileKeys * 128, 1024, 2);
+        const uint32_t pa = td + (i & 1) * kTileKeys;
+        if (lane == 0) {
 #pragma unroll
-        for (int k = 0; k < kTileKeys / 16; ++k)
-          tc_mma_ts(td + kColO, pa + k * 8, bd + k * (16 * 128 >> 4), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
-        tc_commit(b_vempty + 8 * st);
-        tc_commit(b_pv);
+          for (int k = 0; k < kTileKeys / 16; ++k)
+            tc_mma_ts(td + kColO, pa + k * 8, bd + k * (16 * 128 >> 4), idesc_o, (t > 0 || k > 0) ? 1u : 0u);
+          tc_commit(b_vempty + 8 * st);
+          tc_commit(b_pv + 8 * (i & 1));
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
     if (!ok && lane == 0) give_up();
     __syncwarp();
   } else if (warp >= 6) {
     // ---------------------------------------------------------------- converters (8-bit caches)
     if constexpr (W::kQuant) {
-      const int ct = tid - 192;  // 0 .. 63: also the key whose scales this thread brings
+      const int ct = tid - 192;  // 0 .. 127; below 64 also the key whose scales this thread brings
       constexpr int kChunks = D / 16;            // 16-byte chunks of a raw row
-      constexpr int kRowsPer = 64 / kChunks;     // rows that the 64 threads cover at a time
+      constexpr int kRowsPer = 128 / kChunks;    // rows that the 128 threads cover at a time
       const int r8 = (ct & 7) | (ct >> 3) / kChunks * 8, ch = (ct >> 3) % kChunks;
       // Converts a raw tile to an operand tile; rows whose bit of `live` is clear become zeros, and with `finite` e4m3's
       // NaN codes too.
@@ -396,43 +415,67 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
         if (!wait(b_rfull + 8 * st, (i / W::NR) & 1) || !wait(b_kempty + 8 * sk, ((i / W::NK) & 1) ^ 1)) return false;
         const unsigned long long live = live_of(st);
         convert(W::kOffRaw + st * 2 * W::kRawBytes, W::kOffK + sk * W::kOpBytes, live, false);
-        // The key's scales; zeros where it is none (its slot of the raw tile was not loaded).
-        const bool is = (live >> ct) & 1ull;
-        const float *rsc = reinterpret_cast<const float *>(smem + W::kOffRawScale + st * 2 * kTileKeys * 4);
-        const float ks = is ? rsc[ct] : 0.f, vs = is ? rsc[kTileKeys + ct] : 0.f;
-        float *sc = reinterpret_cast<float *>(smem + W::kOffScale + slot * W::kSlotBytes);
-        sc[ct] = ks, sc[kTileKeys + ct] = vs;
-        // Above log2 of the V scale: its exponent + 1, and the largest of the warp's keys.
-        const int ve = static_cast<int>(__float_as_uint(vs) >> 23 & 0xFFu) - 126;
-        sc[2 * kTileKeys + ct] = static_cast<float>(ve);
-        const int top = __reduce_max_sync(0xffffffffu, ve);
-        if (lane == 0) sc[3 * kTileKeys + (warp - 6)] = static_cast<float>(top);
-        if (ct == 0) {
-          st_shared_u32(live_slot + 8 * slot, static_cast<uint32_t>(live));
-          st_shared_u32(live_slot + 8 * slot + 4, static_cast<uint32_t>(live >> 32));
+        if (ct < kTileKeys) {
+          // The key's scales; zeros where it is none (its slot of the raw tile was not loaded).
+          const bool is = (live >> ct) & 1ull;
+          const float *rsc = reinterpret_cast<const float *>(smem + W::kOffRawScale + st * 2 * kTileKeys * 4);
+          const float ks = is ? rsc[ct] : 0.f, vs = is ? rsc[kTileKeys + ct] : 0.f;
+          float *sc = reinterpret_cast<float *>(smem + W::kOffScale + slot * W::kSlotBytes);
+          sc[ct] = ks, sc[kTileKeys + ct] = vs;
+          // Above log2 of the V scale: its exponent + 1, and the largest and smallest of the warp's keys. Rows of zeros (and
+          // of less than e4m3 holds of fp32's smallest) have the smallest scale and no say.
+          const int ve = static_cast<int>(__float_as_uint(vs) >> 23 & 0xFFu) - 126;
+          sc[2 * kTileKeys + ct] = static_cast<float>(ve);
+          const int hi = __reduce_max_sync(0xffffffffu, ve), lo = __reduce_min_sync(0xffffffffu, ve <= -125 ? 1 << 10 : ve);
+          if (lane == 0)
+            sc[3 * kTileKeys + (warp - 6)] = static_cast<float>(hi), sc[3 * kTileKeys + 2 + (warp - 6)] = static_cast<float>(lo);
+          if (ct == 0) {
+            st_shared_u32(live_slot + 8 * slot, static_cast<uint32_t>(live));
+            st_shared_u32(live_slot + 8 * slot + 4, static_cast<uint32_t>(live >> 32));
+          }
         }
         arrive(b_kfull + 8 * sk);
         return true;
       };
       // K of the next tile goes before V of this one: its product is wanted first, and V's buffer is only free once P V of
       // the tile before is done.
-      bool ok = tiles == 0 || convert_k(0);
-      for (int i = 0; i < tiles && ok; ++i) {
-        if (i + 1 < tiles) ok = convert_k(i + 1);
-        const int st = i % W::NR, sv = i % W::NV;
-        ok = ok && wait(b_vempty + 8 * sv, ((i / W::NV) & 1) ^ 1);
-        if (!ok) break;
-        convert(W::kOffRaw + st * 2 * W::kRawBytes + W::kRawBytes, W::kOffV + sv * W::kOpBytes, live_of(st),
-                hides && js + (i + 1) * kTileKeys > open);
-        arrive(b_vfull + 8 * sv);
-        arrive(b_rempty + 8 * st);
+      bool ok = convert_k(0);
+      const int total = u1 - u0;
+      int i = 0;
+      for (; seg.n > 0 && ok; next()) {
+        const bool hides = hides_keys();
+        for (int t = 0; t < seg.n; ++t, ++i) {
+          if (i + 1 < total) ok = convert_k(i + 1);
+          const int st = i % W::NR, sv = i % W::NV;
+          ok = ok && wait(b_vempty + 8 * sv, ((i / W::NV) & 1) ^ 1);
+          if (!ok) break;
+          convert(W::kOffRaw + st * 2 * W::kRawBytes + W::kRawBytes, W::kOffV + sv * W::kOpBytes, live_of(st),
+                  hides && first_key() + (t + 1) * kTileKeys > open_below());
+          arrive(b_vfull + 8 * sv);
+          arrive(b_rempty + 8 * st);
+        }
       }
       if (!ok) give_up();
     }
   } else {
     // ---------------------------------------------------------------- softmax: thread = row
-    const int r = row0 + tid, qi_raw = r / p.group;
-    const int qi = r < p.rows && qi_raw < drafts ? qi_raw : -1;
+    bool ok = true;
+    int i = 0;  // tile of the CTA
+    uint32_t met = 0;
+    auto meet = [&]() {  // a barrier of the four softmax warps, bounded as every wait
+      arrive(b_meet);
+      return wait(b_meet, met++ & 1);
+    };
+    for (; seg.n > 0 && ok; next()) {
+    const int b = seg.b, h = seg.unit / seg.s.blocks, row0 = (seg.unit - h * seg.s.blocks) * kUnitRows;
+    const int nrows = min(kUnitRows, p.rows - row0), L = seg.s.L, drafts = seg.s.drafts, ctx = context();
+    const int js = first_key(), je = static_cast<int>(end_key()), open = open_below();
+    const bool hides = hides_keys();
+    const int32_t *bt = table_of();
+    float m = -INFINITY, l = 0.f, M = -INFINITY;
+    const int vrow = tid % kUnitRows, r = row0 + vrow, qi_raw = r / p.group;
+    const int qi = vrow < nrows && qi_raw < drafts ? qi_raw : -1;
+    const int col0 = tid / kUnitRows * 32;  // REP = 2: the first of the thread's 32 columns (the same for a whole warp)
     const bool warp_live = __any_sync(0xffffffffu, qi >= 0);
     // The query row into shared memory (128-byte swizzled rows, two sub-tiles of 64 elements at head_dim 128). 8-bit
     // caches: brought to fp16 by an exact power of two (see cache_attention.cu), which the scores give back.
@@ -522,10 +565,10 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
     // Up to 64 new tokens: the row's whole mask, fetched here, while the first tiles are on their way.
     const unsigned long long mask64 = p.mask && p.n <= 64 && je > open ? gather(0) : 0ull;
     const uint32_t lanes = static_cast<uint32_t>(warp) << 21;  // TMEM lane 32 * warp
-    bool ok = true;
-    for (int i = 0; i < tiles; ++i) {
+    float vhi = -INFINITY, vlo = INFINITY;  // over the segment's tiles so far: largest and smallest bound of a V scale
+    for (int t = 0; t < seg.n; ++t, ++i) {
       const uint32_t s_addr = tmem + lanes + (i & 1) * kTileKeys;
-      const int slot = i % W::kSlots, j0 = js + i * kTileKeys;
+      const int slot = i % W::kSlots, j0 = js + t * kTileKeys;
       ok = wait(b_sfull + 8 * (i & 1), (i >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
@@ -581,22 +624,23 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
           if (qi < 0) see = 0ull;
           see_lo = lo & static_cast<uint32_t>(see), see_hi = hi & static_cast<uint32_t>(see >> 32);
         }
-        // Scores of columns c0 .. c0 + CW before the row's factor rs > 0. 8-bit caches read S twice, 32 columns at a time
-        // (for the maximum, then for the weights): a tile's 64 scores beside three numbers per key do not fit the
-        // registers of a thread, and what is spilled goes to the L2, the L1 being all shared memory here.
-        constexpr int CW = W::kQuant ? 32 : 64;
+        // Scores of columns c0 .. c0 + CW before the row's factor rs > 0. 8-bit caches with 128 rows read S twice, 32 columns
+        // at a time (for the maximum, then for the weights): a tile's 64 scores beside three numbers per key do not fit
+        // the registers of a thread, and what is spilled goes to the L2, the L1 being all shared memory here.
+        constexpr int CW = W::kQuant || REP == 2 ? 32 : 64;
+        constexpr int kCols = kTileKeys / REP;  // of this thread
+        const int first = REP == 2 ? col0 : 0;
         float x[CW];
         auto scores = [&](int c0) {
+          if constexpr (CW == 32) tmem_ld32(s_addr + c0, x);
+          else tmem_ld64(s_addr, x);
           if constexpr (W::kQuant) {
-            tmem_ld32(s_addr + c0, x);
 #pragma unroll
             for (int c = 0; c < CW; c += 4) {
-              const float4 k4 = sc[(c0 + c) / 4];
+              const float4 k4 = sc[c0 / 4 + c / 4];
               mul2(x[c], x[c + 1], k4.x, k4.y);
               mul2(x[c + 2], x[c + 3], k4.z, k4.w);
             }
-          } else {
-            tmem_ld64(s_addr, x);
           }
           if (edge) {
 #pragma unroll
@@ -608,7 +652,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
         };
         float top = -INFINITY;
 #pragma unroll 1
-        for (int c0 = 0; c0 < kTileKeys; c0 += CW) {
+        for (int c0 = first; c0 < first + kCols; c0 += CW) {
           scores(c0);
           float mx = fmax3(top, x[0], x[1]), mx1 = fmaxf(x[2], x[3]);
 #pragma unroll
@@ -617,14 +661,21 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
         }
         top *= rs;  // the tile's largest score
         const float mt = fmaxf(m, top);
-        // The weights' reference: while the tile's largest score and its largest V scale together stay below M + 8 no
-        // weight can exceed it; only otherwise is the row's own maximum taken.
+        // The weights' reference M. While the row scales of V stay within 2^8 of each other it is the running maximum plus
+        // the bound of the largest one: no weight exceeds it, and fp16 holds the smallest ones' weights to 2^-17 of it. Once
+        // they do not, and in tiles with keys that a row may not see (and must not notice), it is the row's own maximum of
+        // score + bound.
         float Mt = M;
         if constexpr (W::kQuant) {
-          const float2 bound = *reinterpret_cast<const float2 *>(sc + 3 * kTileKeys / 4);
-          if (__any_sync(0xffffffffu, top + fmaxf(bound.x, bound.y) > M + 8.f || M == -INFINITY)) {
+          if (!edge) {
+            const float4 bound = sc[3 * kTileKeys / 4];  // largest (two), smallest (two)
+            vhi = fmax3(vhi, bound.x, bound.y), vlo = fminf(vlo, fminf(bound.z, bound.w));
+          }
+          if (!edge && vhi - vlo <= 8.f) {
+            Mt = mt + vhi;
+          } else if (edge || __any_sync(0xffffffffu, mt + vhi > M + 8.f || M == -INFINITY)) {
 #pragma unroll 1
-            for (int c0 = 0; c0 < kTileKeys; c0 += CW) {
+            for (int c0 = first; c0 < first + kCols; c0 += CW) {
               scores(c0);
 #pragma unroll
               for (int c = 0; c < CW; c += 4) {
@@ -643,8 +694,8 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
           const float ao = W::kQuant ? (Mn == -INFINITY ? 1.f : ex2_approx_ftz(M - Mn)) : al;
           m = mn, M = Mn;
           l *= al;
-          if (i > 0) {
-            ok = wait(b_pv, (i - 1) & 1);  // P V of the tile before is done: O is at rest
+          if (t > 0) {
+            ok = wait(b_pv + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1);  // P V of the tile before is done: O is at rest
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -661,8 +712,8 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
         const float cw = W::kQuant ? ex2_approx_ftz(mu - (M == -INFINITY ? 0.f : M)) : 1.f;
         uint64_t sum0 = 0, sum1 = 0;  // pairs of fp32
 #pragma unroll 1
-        for (int c0 = 0; c0 < kTileKeys; c0 += CW) {
-          if constexpr (W::kQuant) scores(c0);
+        for (int c0 = first; c0 < first + kCols; c0 += CW) {
+          if constexpr (kCols > CW) scores(c0);
 #pragma unroll
           for (int h0 = 0; h0 < CW; h0 += 32) {
             uint32_t pk[16];
@@ -673,7 +724,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
               for (int e = 0; e < 4; ++e) w[e] = ex2_approx_ftz(fmaf(x[h0 + c + e], rs, -mu));
               sum0 = f32x2_add(sum0, f32x2_pack(w[0], w[1])), sum1 = f32x2_add(sum1, f32x2_pack(w[2], w[3]));
               if constexpr (W::kQuant) {
-                const float4 v4 = sc[(kTileKeys + c0 + c) / 4];
+                const float4 v4 = sc[(kTileKeys + c0) / 4 + c / 4];
                 mul2(w[0], w[1], v4.x, v4.y), mul2(w[0], w[1], cw, cw);
                 mul2(w[2], w[3], v4.z, v4.w), mul2(w[2], w[3], cw, cw);
               }
@@ -689,6 +740,10 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
             tmem_st16(s_addr + (c0 + h0) / 2, pk);  // over scores that have been read
           }
         }
+        if constexpr (REP == 2) {  // the other lane's columns
+          const uint32_t none[16] = {};
+          tmem_st16(s_addr + (32 - col0) / 2, none);
+        }
         const float2 sum = f32x2_unpack(f32x2_add(sum0, sum1));
         l += sum.x + sum.y;
         tmem_st_wait();
@@ -696,99 +751,90 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
       tc_fence_before();
       arrive(b_pready + 8 * (i & 1));
     }
-    if (ok && tiles > 0) ok = wait(b_pv, (tiles - 1) & 1);
-    if (!ok) give_up();
+    if (ok) ok = wait(b_pv + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1);
+    if (!ok) break;
     tc_fence_after();
-  }
-  __syncthreads();  // every MMA, copy and conversion of this CTA is done
-  if (p.splits > 1) {
-    cluster_arrive();
-    cluster_wait();  // ... and of the others: their shared memory takes records now
-  }
 
-  // y: 8 finished values of columns d .. d + 7 of CTA row r.
-  auto write8 = [&](int r, int d, float (&y)[8], bool flag) {
-    const int row = row0 + r, qi = row / p.group, gq = row - qi * p.group;
-    if (qi >= drafts) {
+    // The rows' results. REP = 2: lane 64 + r's half joins lane r's, through the query rows' shared memory (every product
+    // that reads them is done): first both halves' references and sums, then the upper half's output.
+    float own = 1.f;  // what this lane's O is multiplied by
+    if constexpr (!W::kQuant) M = m;
+    if constexpr (REP == 2) {
+      float *x = reinterpret_cast<float *>(smem);
+      x[tid * 4] = m, x[tid * 4 + 1] = l, x[tid * 4 + 2] = M;
+      if (!(ok = meet())) break;
+      const float *y = x + (tid ^ kUnitRows) * 4;
+      const float om = y[0], ol = y[1], oM = y[2];
+      if (!(ok = meet())) break;
+      const float mx = fmaxf(m, om), Mx = fmaxf(M, oM);
+      const float mu = mx == -INFINITY ? 0.f : mx, Mu = Mx == -INFINITY ? 0.f : Mx;
+      own = exp2f(M - Mu);
+      l = l * exp2f(m - mu) + ol * exp2f(om - mu);
+      m = mx, M = Mx;
+      uint8_t *half = smem + vrow * D * 4;
+      if (tid >= kUnitRows) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = 0.f;
-    } else if (CT != kI8 && flag) {
-      for (int e = 0; e < 8; ++e) y[e] = add_nonfinite<CT>(p, bt, b, h, qi, d + e, ctx, L, drafts, y[e]);
-    }
-    uint4 u;
-    if (W::kQuant ? p.q_is_f16 : CT == kF16)
-      u = make_uint4(pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]), pack_f16x2(y[6], y[7]));
-    else
-      u = pack8(y);
-    const int64_t idx = ((static_cast<int64_t>(b) * p.n + qi) * p.hq + h * p.group + gq) * D + d;
-    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + idx) = u;
-  };
-  auto finish = [&](float l, float m, float M) {  // what an unnormalised output is multiplied by
-    return l == 0.f ? 0.f : (W::kQuant ? exp2f(M - m) : 1.f) / l;
-  };
-  if constexpr (!W::kQuant) M = m;
-  float *rec = reinterpret_cast<float *>(smem);  // [rows of this CTA][splits][kStride]
-  if (warp < 4) {
-    const uint32_t lanes = static_cast<uint32_t>(warp) << 21;
-    const float f = finish(l, m, M);
-    const bool flagged = ld_shared_u32(dirty) != 0u;
-    const uint32_t to = map_shared_to(
-        smem_addr(rec + ((tid / p.splits) * p.splits + static_cast<int>(rank)) * W::kStride), p.splits > 1 ? tid % p.splits : rank);
+        for (int c = 0; c < D; c += 32) {
+          float t[32];
+          tmem_ld32(tmem + lanes + kColO + c, t);
 #pragma unroll
-    for (int c = 0; c < D; c += 32) {
-      float t[32];
-      if (tiles > 0) {
-        tmem_ld32(tmem + lanes + kColO + c, t);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) t[e] = 0.f;
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4 *>(half + (((c + e) / 4) ^ (vrow & 7)) * 16) =
+                make_float4(t[e] * own, t[e + 1] * own, t[e + 2] * own, t[e + 3] * own);
+        }
       }
-      if (tid < nrows) {
-        if (p.splits == 1) {
+      if (!(ok = meet())) break;
+    }
+    const bool whole = seg.n == seg.s.tiles;
+    const bool flagged = ld_shared_u32(dirty) != 0u;
+    if (tid < kUnitRows) {
+      const int gq = r - qi_raw * p.group;
+      const float f = l == 0.f ? 0.f : (W::kQuant ? exp2f(M - m) : 1.f) / l;
+      float *rec = p.records + (static_cast<int64_t>(record_slot(blockIdx.x, seg.unit_u, T, G)) * kUnitRows + vrow) * (D + 4);
+      const int64_t row = ((static_cast<int64_t>(b) * p.n + qi_raw) * p.hq + h * p.group + gq) * D;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float t[32];
+        tmem_ld32(tmem + lanes + kColO + c, t);
+        if constexpr (REP == 2) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 o = *reinterpret_cast<const float4 *>(smem + vrow * D * 4 + (((c + e) / 4) ^ (vrow & 7)) * 16);
+            t[e] = fmaf(t[e], own, o.x), t[e + 1] = fmaf(t[e + 1], own, o.y);
+            t[e + 2] = fmaf(t[e + 2], own, o.z), t[e + 3] = fmaf(t[e + 3], own, o.w);
+          }
+        }
+        if (vrow < nrows && whole) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             float y[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = t[e + k] * f;
-            write8(tid, c + e, y, flagged);
+            for (int k = 0; k < 8; ++k) y[k] = qi < 0 ? 0.f : t[e + k] * f;
+            if (CT != kI8 && flagged && qi >= 0) {
+              for (int k = 0; k < 8; ++k) y[k] = add_nonfinite<CT>(p, bt, b, h, qi, c + e + k, ctx, L, drafts, y[k]);
+            }
+            uint4 u;
+            if (W::kQuant ? p.q_is_f16 : CT == kF16)
+              u = make_uint4(pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]), pack_f16x2(y[6], y[7]));
+            else
+              u = pack8(y);
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + row + c + e) = u;
           }
-        } else {
+        } else if (vrow < nrows) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) st_cluster_v4(to + (c + e) * 4, t[e], t[e + 1], t[e + 2], t[e + 3]);
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4 *>(rec + c + e) = make_float4(t[e], t[e + 1], t[e + 2], t[e + 3]);
         }
       }
+      if (vrow < nrows && !whole) *reinterpret_cast<float4 *>(rec + D) = make_float4(m, l, M, flagged ? 1.f : 0.f);
     }
-    if (p.splits > 1 && tid < nrows) st_cluster_v4(to + D * 4, m, l, M, flagged ? 1.f : 0.f);
+    tc_fence_before();
+    if constexpr (REP == 2) ok = meet();  // the next segment's query rows go where the halves met
+    }
+    if (!ok) give_up();
   }
   tc_fence_before();
-  if (p.splits > 1) {
-    cluster_arrive();
-    cluster_wait();
-    for (int e = tid; e < (nrows + p.splits - 1) / p.splits * (D / 8); e += W::kThreads) {
-      const int q = e / (D / 8), d = (e - q * (D / 8)) * 8, r = q * p.splits + static_cast<int>(rank);
-      if (r >= nrows) continue;
-      const float *x = rec + q * p.splits * W::kStride;
-      float mx = -INFINITY, Mx = -INFINITY, flag = 0.f, sum = 0.f, y[8] = {};
-      for (int s = 0; s < p.splits; ++s) {
-        mx = fmaxf(mx, x[s * W::kStride + D]);
-        Mx = fmaxf(Mx, x[s * W::kStride + D + 2]);
-        flag = fmaxf(flag, x[s * W::kStride + D + 3]);
-      }
-      const float mu = mx == -INFINITY ? 0.f : mx, Mu = Mx == -INFINITY ? 0.f : Mx;
-      for (int s = 0; s < p.splits; ++s) {
-        const float *w = x + s * W::kStride;
-        const float al = exp2f(w[D] - mu), ao = exp2f(w[D + 2] - Mu);
-        sum = fmaf(al, w[D + 1], sum);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = fmaf(ao, w[d + k], y[k]);
-      }
-      const float f = finish(sum, mx, Mx);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] *= f;
-      write8(r, d, y, flag != 0.f);
-    }
-  }
-  __syncthreads();
+  __syncthreads();  // every MMA, copy and read of this CTA is done
   if (warp == 5) tmem_dealloc(tmem, kTmemCols);
 }
 
@@ -817,43 +863,55 @@ bool make_cache_map(CUtensorMap *map, const void *base, const CacheAttnParams &p
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int wide_splits(int64_t units, int64_t max_keys) {
-  const int64_t want = (2 * static_cast<int64_t>(sm_count()) + units - 1) / units;
-  const int64_t most = std::max<int64_t>(1, max_keys / (4 * kTileKeys));
-  const int64_t s = std::min<int64_t>(std::min(want, most), kMaxSplits);
-  int pow2 = 1;
-  while (pow2 * 2 <= s) pow2 *= 2;
-  return pow2;
+int wide_rows(const CacheAttnParams &p) { return p.rows <= 64 ? 64 : 128; }  // of a unit
+
+// CTAs: as many as run at once, fewer where the longest possible sequences could not feed them.
+int wide_grid(const CacheAttnParams &p) {
+  const int64_t units = static_cast<int64_t>(p.batch) * p.hkv * ((p.rows + wide_rows(p) - 1) / wide_rows(p));
+  const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.block_size + kTileKeys - 1) / kTileKeys;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * sm_count(), std::max(units, units * tiles / kMinTiles))));
 }
 
-template <int CT, int D> int launch_wide(WideParams &wp, const WideMaps &maps, int batch, int num_splits, cudaStream_t s) {
+template <int CT, int D, int REP> int launch_wide(const WideParams &wp, const WideMaps &maps, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};  // bit: device whose shared-memory limit is set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NVB200_ERR_CUDA;
   if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
-    if (cudaFuncSetAttribute(cache_attention_wide_kernel<CT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(cache_attention_wide_kernel<CT, D, REP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kWideSmem) != cudaSuccess) {
       cudaGetLastError();
       return NVB200_ERR_CUDA;
     }
     ready.fetch_or(uint64_t{1} << dev, std::memory_order_release);
   }
-  CacheAttnParams &p = wp.a;
-  const int64_t y = static_cast<int64_t>((p.rows + kTileRows - 1) / kTileRows) * p.hkv;
-  if (y > 65535 || batch > 65535) return NVB200_ERR_UNSUPPORTED;
-  p.splits = num_splits > 0 ? num_splits : wide_splits(y * batch, static_cast<int64_t>(p.max_pages) * p.block_size);
-  return launch_ex(cache_attention_wide_kernel<CT, D>, dim3(p.splits, static_cast<unsigned>(y), batch),
-                   dim3(Wide<CT, D>::kThreads), kWideSmem, s, p.splits, false, wp, maps);
+  const int grid = wide_grid(wp.a);
+  if (int rc = launch_ex(cache_attention_wide_kernel<CT, D, REP>, dim3(grid), dim3(Wide<CT, D>::kThreads), kWideSmem, s, 1,
+                         false, wp, maps))
+    return rc;
+  return launch_cache_attention_merge(wp.a, CT, D, kTileKeys, kTileRows / REP, kMinTiles, grid, s);
+}
+
+template <int CT, int D> int launch_rep(const WideParams &wp, const WideMaps &maps, cudaStream_t s) {
+  return wide_rows(wp.a) == 64 ? launch_wide<CT, D, 2>(wp, maps, s) : launch_wide<CT, D, 1>(wp, maps, s);
 }
 
 }  // namespace
 
-int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, int batch, int num_splits,
-                                cudaStream_t stream) {
-  // Boxes are runs of tokens of one page: 8 rows is the swizzle's period. A zero scale leaves the running maximum of
-  // masked scores undefined here (0 * -inf); the narrow kernel scales before it masks.
+bool wide_takes(const CacheAttnParams &p) {
+  // Boxes are runs of tokens of one page: 8 rows is the swizzle's period. A zero scale would make masked scores 0 * -inf.
   if (p.block_size % 8 != 0 || p.num_blocks > INT32_MAX || !aligned16(p.out) || !(std::fabs(p.scale_log2) > 1e-30f))
-    return NVB200_ERR_UNSUPPORTED;
+    return false;
+  // Tiles are counted in 32 bits.
+  const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.block_size + kTileKeys - 1) / kTileKeys;
+  const int64_t units = static_cast<int64_t>(p.hkv) * ((p.rows + wide_rows(p) - 1) / wide_rows(p)) * p.batch;
+  return units <= INT32_MAX / std::max<int64_t>(tiles, 1);
+}
+
+int64_t wide_workspace_bytes(const CacheAttnParams &p, int head_dim) {
+  return 2ll * wide_grid(p) * wide_rows(p) * (head_dim + 4) * 4;
+}
+
+int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, cudaStream_t stream) {
   WideParams wp{p, 64, p.scale_log2 < 0.f ? -1.f : 1.f};
   while (p.block_size % wp.box_rows != 0) wp.box_rows /= 2;
   wp.a.scale_log2 = std::fabs(p.scale_log2);
@@ -862,14 +920,10 @@ int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, 
       !make_cache_map(&maps.v, p.v_cache, p, ct, head_dim, wp.box_rows))
     return NVB200_ERR_UNSUPPORTED;
   switch (ct) {
-    case kBf16: return head_dim == 64 ? launch_wide<kBf16, 64>(wp, maps, batch, num_splits, stream)
-                                      : launch_wide<kBf16, 128>(wp, maps, batch, num_splits, stream);
-    case kF16: return head_dim == 64 ? launch_wide<kF16, 64>(wp, maps, batch, num_splits, stream)
-                                     : launch_wide<kF16, 128>(wp, maps, batch, num_splits, stream);
-    case kE4M3: return head_dim == 64 ? launch_wide<kE4M3, 64>(wp, maps, batch, num_splits, stream)
-                                      : launch_wide<kE4M3, 128>(wp, maps, batch, num_splits, stream);
-    default: return head_dim == 64 ? launch_wide<kI8, 64>(wp, maps, batch, num_splits, stream)
-                                   : launch_wide<kI8, 128>(wp, maps, batch, num_splits, stream);
+    case kBf16: return head_dim == 64 ? launch_rep<kBf16, 64>(wp, maps, stream) : launch_rep<kBf16, 128>(wp, maps, stream);
+    case kF16: return head_dim == 64 ? launch_rep<kF16, 64>(wp, maps, stream) : launch_rep<kF16, 128>(wp, maps, stream);
+    case kE4M3: return head_dim == 64 ? launch_rep<kE4M3, 64>(wp, maps, stream) : launch_rep<kE4M3, 128>(wp, maps, stream);
+    default: return head_dim == 64 ? launch_rep<kI8, 64>(wp, maps, stream) : launch_rep<kI8, 128>(wp, maps, stream);
   }
 }
 

@@ -32,7 +32,7 @@ EXPORTS = ("nvb200_status_string", "nvb200_qk_norm_rope_kv", "nvb200_qk_norm_rop
            "nvb200_paged_decode_attention", "nvb200_paged_decode_splits", "nvb200_paged_decode_workspace_size",
            "nvb200_paged_decode_attention_streamk", "nvb200_paged_decode_attention_noalloc",
            "nvb200_store_kvcache_quant", "nvb200_qk_norm_rope_kv_quant", "nvb200_load_kvcache_quant",
-           "nvb200_cache_attention")
+           "nvb200_cache_attention_workspace_size", "nvb200_cache_attention")
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
 
@@ -163,7 +163,9 @@ def _declare(lib):
     lib.nvb200_load_kvcache_quant.argtypes = [_vp, _vp, ctypes.POINTER(QuantCache), _vp, _i64, _i32, _vp, _i32, _i64,
                                               ctypes.c_int, ctypes.c_int, _vp, _vp]
     lib.nvb200_load_kvcache_quant.restype = ctypes.c_int
-    lib.nvb200_cache_attention.argtypes = [ctypes.POINTER(CacheAttentionArgs), _vp]
+    lib.nvb200_cache_attention_workspace_size.argtypes = [ctypes.POINTER(CacheAttentionArgs)]
+    lib.nvb200_cache_attention_workspace_size.restype = _i64
+    lib.nvb200_cache_attention.argtypes = [ctypes.POINTER(CacheAttentionArgs), _vp, _i64, _vp]
     lib.nvb200_cache_attention.restype = ctypes.c_int
 
 

@@ -6,7 +6,8 @@
 * `decode_attention_quant`: `attention.decode_attention` (single tokens or a causal chain) over an 8-bit cache.
 
 The new tokens' keys and values are in the cache already (its last rows). Both launch on the current stream of q's
-device, allocate their output with torch (graph-capture safe), keep no workspace, and never read device data on the host.
+device, allocate their output and workspace with torch (graph-capture safe; nothing is kept between calls), and never read
+device data on the host.
 Out-of-range block-table entries and lengths are never followed; they are flagged in the device status word
 (nanovllm_b200.status()). Types and layouts without a kernel raise NotImplementedError.
 """
@@ -89,8 +90,11 @@ def _run(what, q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table
         scales[0], scales[1], nb, table, table_stride, seqlens.data_ptr(), _lib.ptr(draft_lens), mask, mask_b, mask_r,
         B, n, hq, hkv, d, bs, pages, int(bool(causal)), int(num_splits), _QUERY[q.dtype], code,
         d ** -0.5 if softmax_scale is None else float(softmax_scale), _lib.status_word(dev).data_ptr())
+    L = _lib.lib()
     with _lib.device_of(dev):
-        rc = _lib.lib().nvb200_cache_attention(a, _lib.stream_of(q))
+        need = L.nvb200_cache_attention_workspace_size(a)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+        rc = L.nvb200_cache_attention(a, _lib.ptr(ws), max(need, 0), _lib.stream_of(q))
     if rc == _lib.ERR_UNSUPPORTED:
         raise NotImplementedError(f"{what}: cache rows must be 16-byte aligned, and a sequence's block table address "
                                   "fewer than 2^31 - 65536 keys")

@@ -120,7 +120,7 @@ def test_refusals():
 def test_entry_point_checks_arguments_without_a_gpu():
     from nanovllm_b200 import _lib
     f = _lib.lib().nvb200_cache_attention
-    assert f(None, None) == _lib.ERR_ARG
+    assert f(None, None, 0, None) == _lib.ERR_ARG
 
     def args(**kw):
         a = _lib.CacheAttentionArgs()
@@ -131,7 +131,8 @@ def test_entry_point_checks_arguments_without_a_gpu():
         a.block_size, a.max_blocks_per_seq, a.dtype, a.cache_dtype, a.softmax_scale = 16, 4, _lib.BF16, _lib.BF16, 0.1
         for k, v in kw.items():
             setattr(a, k, v)
-        return f(a, None)
+        assert (_lib.lib().nvb200_cache_attention_workspace_size(a) == -1) == (f(a, None, 0, None) in (_lib.ERR_ARG, _lib.ERR_UNSUPPORTED))
+        return f(a, None, 0, None)
     for bad in (dict(num_q_heads=3), dict(num_kv_heads=0), dict(batch=-1), dict(block_size=0), dict(causal=2),
                 dict(num_splits=9), dict(num_splits=-1), dict(dtype=_lib.F32), dict(cache_dtype=_lib.F16), dict(q=None),
                 dict(softmax_scale=float("nan")), dict(cache_dtype=_lib.E4M3, k_scale=None), dict(seqlens=None),
