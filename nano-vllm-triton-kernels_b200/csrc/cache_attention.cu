@@ -72,9 +72,13 @@ template <int CT, int D, int NT> struct Geometry {
   static constexpr int kStageBytes = 2 * kKvBytes + kScaleBytes + 128;  // a multiple of 128
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kStride = D + 4;  // floats per record: o[D], m, l, M, flag
-  static constexpr int kRecords = kWarps * kRows * kStride * 4;
+  static constexpr int kRecs = NT == 4 ? 2 : kWarps;  // warps' records in shared memory at once
+  static constexpr int kRecords = kRecs * kRows * kStride * 4;
+  // 32 rows: the query fragments (and the rows' factors) do not fit the registers beside the output and live in shared memory,
+  // [D / 16][2][32 lanes] of 16 bytes, as the lanes take them.
+  static constexpr int kQBytes = NT == 4 ? D / 16 * 2 * 32 * 16 + kRows * 4 : 0;
   static constexpr int kPartials = (kMaxSplits + kRows - 1) * kStride * 4;  // splits * ceil(kRows / splits) records
-  static constexpr int kSmem = kRing + kRecords;
+  static constexpr int kSmem = kRing + kRecords + kQBytes;
   static_assert(kPartials <= kRing, "a cluster's records take the ring's place");
   static constexpr int kCtasPerSm = 228 * 1024 / (kSmem + 1024) >= 3 ? 3 : 2;
   // Physical 16-byte chunk of logical chunk c of row r: the 8 rows of an 8 x 16-byte matrix at one logical chunk fall
@@ -97,6 +101,13 @@ template <int D, int NT> struct RowState {
     }
   }
 };
+
+// Query fragments (second operand of K Q^T) and what the scores of rows 8 n + 2 t + e are multiplied by.
+template <int D, int NT> struct QueryFrags {
+  uint32_t b[D / 16][NT][2];
+  float rs[NT][2];
+};
+template <int D> struct QueryFrags<D, 4> {};  // in shared memory
 
 // Replaces every infinity and NaN of the V tile by zero; true if there were any (in any lane).
 template <int CT, int D, int NT> NVB200_DEVICE bool clean_v_tile(uint32_t kt, int lane) {
@@ -121,8 +132,8 @@ template <int CT, int D, int NT> NVB200_DEVICE bool clean_v_tile(uint32_t kt, in
 // Folds one tile. kt: the stage's base address. see[n][e]: which of the tile's keys that row sees, where `edge`; elsewhere
 // every row sees every key.
 template <int CT, int D, int NT>
-NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const uint32_t (&qb)[D / 16][NT][2],
-                             const float (&rs)[NT][2], int lane, bool edge, const uint32_t (&see)[NT][2]) {
+NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<D, NT> &q, const uint4 *qs,
+                             const float *rs_s, int lane, bool edge, const uint32_t (&see)[NT][2]) {
   using G = Geometry<CT, D, NT>;
   using C = CacheType<CT>;
   constexpr int KB = G::kTile / 16;  // 16-key blocks
@@ -132,30 +143,53 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const uint32_t (&
   for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[kb][n][0] = s[kb][n][1] = s[kb][n][2] = s[kb][n][3] = 0.f;
-    const int key = kb * 16 + (mq & 1) * 8 + rr;
-    const uint32_t row = kt + key * G::kRowBytes;
-    if constexpr (!C::kQuant) {
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t a[4];
-        ldsm_x4(row + G::chunk(key, 2 * ks + (mq >> 1)) * 16, a);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma_ct<CT>(s[kb][n], a, qb[ks][n][0], qb[ks][n][1]);
-      }
+  }
+  // Query fragments of k-step ks.
+  uint32_t qk[NT][2];
+  auto load_q = [&](int ks) {
+    if constexpr (NT == 4) {
+      const uint4 x = qs[(2 * ks) * 32 + lane], y = qs[(2 * ks + 1) * 32 + lane];
+      qk[0][0] = x.x, qk[0][1] = x.y, qk[1][0] = x.z, qk[1][1] = x.w;
+      qk[2][0] = y.x, qk[2][1] = y.y, qk[3][0] = y.z, qk[3][1] = y.w;
     } else {
-      // A matrix is 8 keys x 16 codes: one k-step of 16, of which lane (g, t) gets key g's codes 4 t .. 4 t + 3. The
-      // instruction's k order (2t, 2t + 1 | 2t + 8, 2t + 9) stands for those four; the query fragments are laid out alike.
 #pragma unroll
-      for (int k2 = 0; k2 < D / 32; ++k2) {
-        uint32_t w[4];
-        ldsm_x4(row + G::chunk(key, 2 * k2 + (mq >> 1)) * 16, w);
+      for (int n = 0; n < NT; ++n) qk[n][0] = q.b[ks][n][0], qk[n][1] = q.b[ks][n][1];
+    }
+  };
+  if constexpr (!C::kQuant) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+    for (int ks = 0; ks < D / 16; ++ks) {
+      load_q(ks);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int key = kb * 16 + (mq & 1) * 8 + rr;
+        uint32_t a[4];
+        ldsm_x4(kt + key * G::kRowBytes + G::chunk(key, 2 * ks + (mq >> 1)) * 16, a);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_ct<CT>(s[kb][n], a, qk[n][0], qk[n][1]);
+      }
+    }
+  } else {
+    // A matrix is 8 keys x 16 codes: one k-step of 16, of which lane (g, t) gets key g's codes 4 t .. 4 t + 3. The
+    // instruction's k order (2t, 2t + 1 | 2t + 8, 2t + 9) stands for those four; the query fragments are laid out alike.
+#pragma unroll
+    for (int k2 = 0; k2 < D / 32; ++k2) {
+      uint32_t w[KB][4];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int key = kb * 16 + (mq & 1) * 8 + rr;
+        ldsm_x4(kt + key * G::kRowBytes + G::chunk(key, 2 * k2 + (mq >> 1)) * 16, w[kb]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        load_q(2 * k2 + i);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
           uint32_t a[4];
-          codes_to_f16<CT>(w[2 * i], a[0], a[2]);
-          codes_to_f16<CT>(w[2 * i + 1], a[1], a[3]);
+          codes_to_f16<CT>(w[kb][2 * i], a[0], a[2]);
+          codes_to_f16<CT>(w[kb][2 * i + 1], a[1], a[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_ct<CT>(s[kb][n], a, qb[2 * k2 + i][n][0], qb[2 * k2 + i][n][1]);
+          for (int n = 0; n < NT; ++n) mma_ct<CT>(s[kb][n], a, qk[n][0], qk[n][1]);
         }
       }
     }
@@ -180,7 +214,10 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const uint32_t (&
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float &x = s[kb][n][2 * i + e];
-          x = C::kQuant ? x * rs[n][e] * ks : x * rs[n][e];
+          float f;
+          if constexpr (NT == 4) f = rs_s[8 * n + 2 * (lane & 3) + e];
+          else f = q.rs[n][e];
+          x = C::kQuant ? x * f * ks : x * f;
           if (edge && !((see[n][e] >> key) & 1u)) x = -INFINITY;
         }
       }
@@ -285,7 +322,9 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t wring = smem_addr(smem) + warp * (G::kStages * G::kStageBytes);
-  float *rec = reinterpret_cast<float *>(smem + G::kRing);  // [kWarps][kRows][kStride]
+  float *rec = reinterpret_cast<float *>(smem + G::kRing);  // [kRecs][kRows][kStride]
+  uint4 *qs = reinterpret_cast<uint4 *>(smem + G::kRing + G::kRecords);
+  float *rs_s = reinterpret_cast<float *>(qs + D / 16 * 2 * 32);
 
   Segment seg;
   int u1, T = 0, ctas = 0;
@@ -306,9 +345,14 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
     T = total_work(p, G::kTile, G::kRows);
     ctas = active_ctas(T, gridDim.x, kMinTiles);
     zero_uncovered_rows(p, D, G::kTile, G::kRows, blockIdx.x, gridDim.x, tid, kThreads);
-    if (T == 0 || static_cast<int>(blockIdx.x) >= ctas) return;
-    u1 = range_start(blockIdx.x + 1, T, ctas);
-    seg = find_segment(p, range_start(blockIdx.x, T, ctas), u1, G::kTile, G::kRows);
+    seg.n = 0;
+    const bool work = T > 0 && static_cast<int>(blockIdx.x) < ctas;
+    if (work) {
+      u1 = range_start(blockIdx.x + 1, T, ctas);
+      seg = find_segment(p, range_start(blockIdx.x, T, ctas), u1, G::kTile, G::kRows);
+    }
+    if (tid == 0) write_cut(p, blockIdx.x, seg, T, ctas);
+    if (!work) return;
   }
   const bool masked = p.mask != nullptr || p.causal;
 
@@ -402,10 +446,10 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
     // order as in fold_tile, the row brought to fp16 by a power of two that puts its largest element in [2^13, 2^14)
     // (bf16's range does not fit fp16; elements below 2^-27 of the largest lose bits, fewer than the fp32 sum would). rs:
     // what the scores of rows 2 t and 2 t + 1 are multiplied by.
-    uint32_t qb[D / 16][NT][2];
-    float rs[NT][2];
+    QueryFrags<D, NT> q;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n0 = 0; n0 < (NT == 4 ? 1 : NT); ++n0) {
+      const int n = NT == 4 ? warp : n0;  // 32 rows: each warp brings one row tile
       const int r = row0 + 8 * n + g, qi = r / p.group;
       const uint16_t *row = r < p.rows ? static_cast<const uint16_t *>(p.q) + b * p.q_batch_stride +
                                              qi * p.q_token_stride +
@@ -451,10 +495,19 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
           }
         }
       }
+      if constexpr (NT == 4) {
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) qb[ks][n][0] = w[ks][0], qb[ks][n][1] = w[ks][1];
-      rs[n][0] = __shfl_sync(0xffffffffu, f, 8 * t), rs[n][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+        for (int ks = 0; ks < D / 16; ++ks)
+          *reinterpret_cast<uint2 *>(reinterpret_cast<uint8_t *>(qs + (2 * ks + (n >> 1)) * 32 + lane) + (n & 1) * 8) =
+              make_uint2(w[ks][0], w[ks][1]);
+        if (t == 0) rs_s[8 * n + g] = f;
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) q.b[ks][n0][0] = w[ks][0], q.b[ks][n0][1] = w[ks][1];
+        q.rs[n0][0] = __shfl_sync(0xffffffffu, f, 8 * t), q.rs[n0][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+      }
     }
+    if constexpr (NT == 4) __syncthreads();
     RowState<D, NT> st;
     st.reset();
 
@@ -510,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
           if (j0 + G::kTile > open && (p.mask ? drafts > 0 : drafts > 1)) dirty |= clean_v_tile<CT, D, NT>(kt, lane);
         }
       }
-      fold_tile<CT, D, NT>(st, kt, qb, rs, lane, edge, see);
+      fold_tile<CT, D, NT>(st, kt, q, qs, rs_s, lane, edge, see);
     }
 
     // The warp's record: o, m, l, M, flag per row.
@@ -518,22 +571,61 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float l = st.l[n][e];
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        float *w = rec + (warp * G::kRows + 8 * n + 2 * t + e) * G::kStride;
+        for (int o = 4; o < 32; o <<= 1) st.l[n][e] += __shfl_xor_sync(0xffffffffu, st.l[n][e], o);
+        if constexpr (!C::kQuant) st.M[n][e] = st.m[n][e];
+      }
+    }
+    auto put_record = [&](int at) {
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          if constexpr (C::kQuant) {
-            *reinterpret_cast<float2 *>(w + 16 * c + 2 * g) = make_float2(st.o[c][n][e], st.o[c][n][2 + e]);
-          } else {
-            w[16 * c + g] = st.o[c][n][e], w[16 * c + 8 + g] = st.o[c][n][2 + e];
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float *w = rec + (at * G::kRows + 8 * n + 2 * t + e) * G::kStride;
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            if constexpr (C::kQuant) {
+              *reinterpret_cast<float2 *>(w + 16 * c + 2 * g) = make_float2(st.o[c][n][e], st.o[c][n][2 + e]);
+            } else {
+              w[16 * c + g] = st.o[c][n][e], w[16 * c + 8 + g] = st.o[c][n][2 + e];
+            }
+          }
+          if (g == 0)
+            *reinterpret_cast<float4 *>(w + D) = make_float4(st.m[n][e], st.l[n][e], st.M[n][e], dirty ? 1.f : 0.f);
+        }
+      }
+    };
+    if constexpr (NT == 4) {
+      // Room for two records: warps 2 and 3 hand theirs to warps 0 and 1.
+      if (warp >= 2) put_record(warp - 2);
+      __syncthreads();
+      if (warp < 2) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float *w = rec + (warp * G::kRows + 8 * n + 2 * t + e) * G::kStride;
+            const float4 x = *reinterpret_cast<const float4 *>(w + D);
+            const float mx = fmaxf(st.m[n][e], x.x), Mx = fmaxf(st.M[n][e], x.z);
+            const float mu = mx == -INFINITY ? 0.f : mx, Mu = Mx == -INFINITY ? 0.f : Mx;
+            const float mine = exp2f(st.M[n][e] - Mu), theirs = exp2f(x.z - Mu);
+            st.l[n][e] = st.l[n][e] * exp2f(st.m[n][e] - mu) + x.y * exp2f(x.x - mu);
+            st.m[n][e] = mx, st.M[n][e] = Mx;
+            dirty |= x.w != 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              const float a0 = C::kQuant ? w[16 * c + 2 * g] : w[16 * c + g];
+              const float a1 = C::kQuant ? w[16 * c + 2 * g + 1] : w[16 * c + 8 + g];
+              st.o[c][n][e] = fmaf(a0, theirs, st.o[c][n][e] * mine);
+              st.o[c][n][2 + e] = fmaf(a1, theirs, st.o[c][n][2 + e] * mine);
+            }
           }
         }
-        if (g == 0)
-          *reinterpret_cast<float4 *>(w + D) =
-              make_float4(st.m[n][e], l, C::kQuant ? st.M[n][e] : st.m[n][e], dirty ? 1.f : 0.f);
+        __syncwarp();
+        put_record(warp);
       }
+    } else {
+      put_record(warp);
     }
     __syncthreads();
 
@@ -555,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
     if constexpr (CLUSTER) {
       if (p.splits == 1) {
         for (int e = tid; e < nrows * D; e += kThreads)
-          write(e / D, e % D, merge(rec + e / D * G::kStride, kWarps, G::kRows * G::kStride, e % D));
+          write(e / D, e % D, merge(rec + e / D * G::kStride, G::kRecs, G::kRows * G::kStride, e % D));
         return;
       }
       // Row r is finished by CTA r mod splits: every CTA sends its merged record there, into the ring's place (the first
@@ -567,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
       cluster_wait();
       for (int e = tid; e < nrows * D; e += kThreads) {
         const int r = e / D, d = e - r * D;
-        const Merged x = merge(rec + r * G::kStride, kWarps, G::kRows * G::kStride, d);
+        const Merged x = merge(rec + r * G::kStride, G::kRecs, G::kRows * G::kStride, d);
         const uint32_t to = map_shared_to(smem_addr(part + ((r / p.splits) * p.splits + rank) * G::kStride), r % p.splits);
         st_cluster_f32(to + d * 4, x.o);
         if (d == 0) {
@@ -587,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
       float *out = p.records + static_cast<int64_t>(record_slot(blockIdx.x, seg.unit_u, T, ctas)) * G::kRows * G::kStride;
       for (int e = tid; e < nrows * D; e += kThreads) {
         const int r = e / D, d = e - r * D;
-        const Merged x = merge(rec + r * G::kStride, kWarps, G::kRows * G::kStride, d);
+        const Merged x = merge(rec + r * G::kStride, G::kRecs, G::kRows * G::kStride, d);
         if (whole) {
           write(r, d, x);
         } else {
@@ -652,27 +744,32 @@ int64_t total_tiles(const CacheAttnParams &p, const NarrowShape &n) {
   return tiles > 0 && units > INT64_MAX / tiles ? INT64_MAX : units * tiles;
 }
 
-// CTAs of the even-share form; 0: the call takes the cluster form. One sequence (or so few units that clusters hold their
-// keys) needs no balancing, and the cluster form is one launch.
+// CTAs of the even-share form; 0: the call takes the cluster form, one launch instead of two, whose CTAs of one sequence are
+// even but whose sequences may not be. That costs at most one sequence's keys, so it stays where the block tables address
+// few (32 sequences of 1024 keys: 17.4 against 25.2 us), where the units fill several waves, and for one sequence, unless it
+// has too few CTAs in its clusters (24 sequences of up to 32768 keys: 197 against 239 us).
+constexpr int kFewKeys = 2048;
 int narrow_grid(const CacheAttnParams &p, const NarrowShape &n, int num_splits) {
   if (num_splits > 0) return 0;
   const int64_t units = n.units * p.batch, slots = static_cast<int64_t>(n.ctas_per_sm) * sm_count();
   const int64_t tiles = total_tiles(p, n);
   if (tiles > INT32_MAX) return 0;  // tiles are counted in 32 bits
-  if (p.batch == 1 && (units * kMaxSplits >= slots / 2 || tiles <= units * kMaxSplits * 2 * kMinTiles)) return 0;
+  if (static_cast<int64_t>(p.max_pages) * p.block_size <= kFewKeys || units >= 4 * slots) return 0;
+  if (p.batch == 1 && units * kMaxSplits >= slots / 2) return 0;
   return static_cast<int>(std::max<int64_t>(1, std::min(slots, std::max(units, tiles / kMinTiles))));
 }
 
-template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_splits, cudaStream_t s) {
+template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_splits, void *workspace, cudaStream_t s) {
   using G = Geometry<CT, D, NT>;
   const NarrowShape n = shape_of<CT, D, NT>(p);
-  const int grid = p.records ? narrow_grid(p, n, num_splits) : 0;
+  const int grid = workspace ? narrow_grid(p, n, num_splits) : 0;
   if (grid > 0) {
+    place_workspace(p, workspace, grid);
     static std::atomic<uint64_t> ready{0};  // bit: device whose shared-memory limit is set
     if (int rc = allow_smem(cache_attention_kernel<CT, D, NT, false>, G::kSmem, ready)) return rc;
     if (int rc = launch_ex(cache_attention_kernel<CT, D, NT, false>, dim3(grid), dim3(kThreads), G::kSmem, s, 1, false, p))
       return rc;
-    return launch_cache_attention_merge(p, CT, D, G::kTile, G::kRows, kMinTiles, grid, s);
+    return launch_cache_attention_merge(p, CT, D, G::kRows, grid, s);
   }
   static std::atomic<uint64_t> ready{0};
   if (int rc = allow_smem(cache_attention_kernel<CT, D, NT, true>, G::kSmem, ready)) return rc;
@@ -682,13 +779,20 @@ template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_s
                    dim3(kThreads), G::kSmem, s, p.splits, false, p);
 }
 
-template <int CT> int launch_dim(CacheAttnParams &p, int d, int num_splits, cudaStream_t s) {
+template <int CT> int launch_dim(CacheAttnParams &p, int d, int num_splits, void *workspace, cudaStream_t s) {
   if (d == 64)
-    return p.rows <= 8 ? launch_narrow<CT, 64, 1>(p, num_splits, s) : launch_narrow<CT, 64, 2>(p, num_splits, s);
-  return p.rows <= 8 ? launch_narrow<CT, 128, 1>(p, num_splits, s) : launch_narrow<CT, 128, 2>(p, num_splits, s);
+    return p.rows <= 8    ? launch_narrow<CT, 64, 1>(p, num_splits, workspace, s)
+           : p.rows <= 16 ? launch_narrow<CT, 64, 2>(p, num_splits, workspace, s)
+                          : launch_narrow<CT, 64, 4>(p, num_splits, workspace, s);
+  return p.rows <= 8    ? launch_narrow<CT, 128, 1>(p, num_splits, workspace, s)
+         : p.rows <= 16 ? launch_narrow<CT, 128, 2>(p, num_splits, workspace, s)
+                        : launch_narrow<CT, 128, 4>(p, num_splits, workspace, s);
 }
 
-constexpr int kNarrowRows = 16;
+#ifndef NVB200_NARROW_ROWS
+#define NVB200_NARROW_ROWS 64
+#endif
+constexpr int kNarrowRows = NVB200_NARROW_ROWS;
 
 // Checks a call and fills `p` (all but the workspace) and *ct; *launch = false where there is nothing to do.
 int prepare_attention(const nvb200_cache_attention_args *a, CacheAttnParams &p, int *ct, bool *launch) {
@@ -751,9 +855,9 @@ extern "C" int64_t nvb200_cache_attention_workspace_size(const nvb200_cache_atte
   bool launch = false;
   if (prepare_attention(a, p, &ct, &launch) != NVB200_OK) return -1;
   if (!launch) return 0;
-  if (p.rows > kNarrowRows && a->num_splits == 0 && wide_takes(p)) return wide_workspace_bytes(p, a->head_dim);
+  if (p.rows > kNarrowRows && a->num_splits == 0 && wide_takes(p)) return wide_workspace_bytes(p, ct, a->head_dim);
   const NarrowShape n = narrow_shape(p, ct, a->head_dim);
-  return 2ll * narrow_grid(p, n, a->num_splits) * n.rows * (a->head_dim + 4) * 4;
+  return even_share_bytes(narrow_grid(p, n, a->num_splits), n.rows, a->head_dim);
 }
 
 extern "C" int nvb200_cache_attention(const nvb200_cache_attention_args *a, void *workspace, int64_t workspace_bytes,
@@ -767,17 +871,17 @@ extern "C" int nvb200_cache_attention(const nvb200_cache_attention_args *a, void
   if (int rc = check_device()) return rc;
   const int64_t need = nvb200_cache_attention_workspace_size(a);
   if (workspace && workspace_bytes < need) return NVB200_ERR_ARG;
-  p.records = need > 0 ? static_cast<float *>(workspace) : nullptr;
+  if (need == 0) workspace = nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (p.rows > kNarrowRows && a->num_splits == 0 && p.records && wide_takes(p)) {
-    const int rc = launch_cache_attention_wide(p, ct, a->head_dim, s);
+  if (p.rows > kNarrowRows && a->num_splits == 0 && workspace && wide_takes(p)) {
+    const int rc = launch_cache_attention_wide(p, ct, a->head_dim, workspace, s);
     if (rc != NVB200_ERR_UNSUPPORTED) return rc;
-    p.records = nullptr;  // sized for the other kernel: the cluster form needs none
+    workspace = nullptr;  // sized for the other kernel: the cluster form needs none
   }
   switch (ct) {
-    case kBf16: return launch_dim<kBf16>(p, a->head_dim, a->num_splits, s);
-    case kF16: return launch_dim<kF16>(p, a->head_dim, a->num_splits, s);
-    case kE4M3: return launch_dim<kE4M3>(p, a->head_dim, a->num_splits, s);
-    default: return launch_dim<kI8>(p, a->head_dim, a->num_splits, s);
+    case kBf16: return launch_dim<kBf16>(p, a->head_dim, a->num_splits, workspace, s);
+    case kF16: return launch_dim<kF16>(p, a->head_dim, a->num_splits, workspace, s);
+    case kE4M3: return launch_dim<kE4M3>(p, a->head_dim, a->num_splits, workspace, s);
+    default: return launch_dim<kI8>(p, a->head_dim, a->num_splits, workspace, s);
   }
 }

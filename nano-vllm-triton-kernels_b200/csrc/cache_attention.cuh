@@ -11,6 +11,15 @@ enum { kBf16 = 0, kF16 = 1, kE4M3 = 2, kI8 = 3 };  // element type of the cache
 
 constexpr int kMaxSplits = 8;  // CTAs sharing one sequence's keys: portable cluster size
 
+// The start of CTA c's range, written by CTA c. A unit is merged by the first end of a range that cuts it.
+struct CutInfo {
+  int parts;  // records of the unit that this end is the first to cut; 0: nothing to merge here
+  int unit_u, T, G;
+  int b, unit, blocks, L;
+  int drafts, pad[3];
+};
+static_assert(sizeof(CutInfo) == 48, "whole 16-byte pieces");
+
 struct CacheAttnParams {
   const void *q;
   int64_t q_batch_stride, q_token_stride, q_head_stride;
@@ -30,7 +39,10 @@ struct CacheAttnParams {
   int n, hq, hkv, group, block_size, bs_shift, max_pages, rows, causal;
   int batch;
   int splits;      // CTAs of a cluster sharing the keys of a sequence (cluster form)
-  float *records;  // workspace of the even-share form: [2 * grid] records of [block_rows][D + 4] floats
+  // Workspace of the even-share form: what each CTA says of the start of its range, then [2 * grid] records of
+  // [block_rows][D + 4] floats.
+  struct CutInfo *cuts;
+  float *records;
   int q_is_f16;
   float scale_log2;
   int32_t *status;
@@ -215,6 +227,18 @@ NVB200_DEVICE int total_work(const CacheAttnParams &p, int tile_keys, int block_
 // CTAs that get work: fewer than are launched when the tiles are few.
 NVB200_DEVICE int active_ctas(int T, int grid, int min_tiles) { return max(1, min(grid, T / min_tiles)); }
 
+// Says what CTA c's start cuts. One thread of every CTA of the grid, those without work included (g.n = 0).
+NVB200_DEVICE void write_cut(const CacheAttnParams &p, int c, const Segment &g, int T, int G) {
+  CutInfo x{};
+  if (g.n > 0 && g.t0 > 0 && range_start(c - 1, T, G) <= g.unit_u) {
+    x.parts = range_owner(g.unit_u + g.s.tiles - 1, T, G) - (c - 1) + 1;
+    x.unit_u = g.unit_u, x.T = T, x.G = G, x.b = g.b, x.unit = g.unit, x.blocks = g.s.blocks, x.L = g.s.L, x.drafts = g.s.drafts;
+  }
+  uint4 *to = reinterpret_cast<uint4 *>(p.cuts + c);
+  const uint4 *from = reinterpret_cast<const uint4 *>(&x);
+  to[0] = from[0], to[1] = from[1], to[2] = from[2];
+}
+
 // Rows of the output that no unit covers (tokens behind draft_lens[b] beyond the last block, sequences without keys):
 // zeros, CTA c of `grid` taking every grid-th sequence. Also reports clamped lengths.
 NVB200_DEVICE void zero_uncovered_rows(const CacheAttnParams &p, int head_dim, int tile_keys, int block_rows, int c, int grid,
@@ -271,11 +295,18 @@ NVB200_DEVICE float add_nonfinite(const CacheAttnParams &p, const int32_t *bt, i
 // The wide kernel (cache_attention_wide.cu). NVB200_ERR_UNSUPPORTED where it does not take the call (pages whose size is
 // not a multiple of 8 tokens, cache strides that no tensor map describes).
 bool wide_takes(const CacheAttnParams &p);
-int64_t wide_workspace_bytes(const CacheAttnParams &p, int head_dim);
-int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, cudaStream_t stream);
+int64_t wide_workspace_bytes(const CacheAttnParams &p, int ct, int head_dim);
+int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, void *workspace, cudaStream_t stream);
 
 // Merges the records of the units that range ends cut, after a grid of `grid` CTAs.
-int launch_cache_attention_merge(const CacheAttnParams &p, int ct, int head_dim, int tile_keys, int block_rows,
-                                 int min_tiles, int grid, cudaStream_t stream);
+int launch_cache_attention_merge(const CacheAttnParams &p, int ct, int head_dim, int block_rows, int grid,
+                                 cudaStream_t stream);
+inline int64_t even_share_bytes(int grid, int block_rows, int head_dim) {
+  return static_cast<int64_t>(grid) * (sizeof(CutInfo) + 2ll * block_rows * (head_dim + 4) * 4);
+}
+inline void place_workspace(CacheAttnParams &p, void *workspace, int grid) {
+  p.cuts = static_cast<CutInfo *>(workspace);
+  p.records = reinterpret_cast<float *>(p.cuts + grid);
+}
 
 }  // namespace nvb200

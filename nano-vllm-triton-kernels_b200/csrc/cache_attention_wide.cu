@@ -29,22 +29,25 @@ constexpr int kTmemCols = 256;  // S: 2 x 64, O: up to 128
 constexpr int kColO = 128;
 constexpr int kPrefetch = 5;  // tiles ahead of the one being loaded that are brought into the L2
 constexpr int kMinTiles = 4;  // of a CTA, where there are too few for all
-// Shared memory of a CTA: exactly two fit on an SM (228 KB, 1 KB of it reserved per CTA). Nothing that holds TMEM fits
-// beside two, so a CTA never waits for TMEM that a CTA of another kernel holds.
-constexpr int kWideSmem = 113 * 1024;
 
 template <int CT, int D> struct Wide {
   static constexpr bool kQuant = CacheType<CT>::kQuant;
   static constexpr int kThreads = kQuant ? 320 : 192;
+  // CTAs per SM. 16-bit caches: two, of 113 KB of shared memory each (228 KB, 1 KB of it reserved per CTA), so that nothing
+  // that holds TMEM fits beside two and a CTA never waits for TMEM that another kernel's CTA holds. 8-bit caches: one with
+  // deep rings; at two per SM the four converting warps beside the softmax leave too few registers, and spilled ones go to
+  // the L2 (the L1 is all shared memory here).
+  static constexpr int kCtas = kQuant ? 1 : 2;
+  static constexpr int kSmem = kQuant ? 227 * 1024 : 113 * 1024;
   static constexpr int kConvWarps = 4;  // one per scheduler
   static constexpr int kQBytes = kTileRows * D * 2;
   static constexpr int kOpBytes = kTileKeys * D * 2;  // a K or V operand tile
   static constexpr int kRawBytes = kTileKeys * D;     // the same as codes
   // Ring depths: K and V operand tiles, pairs of raw tiles, slots of per-key information.
-  static constexpr int NK = kQuant ? 1 : (D == 128 ? 2 : 4);
-  static constexpr int NV = kQuant ? 1 : (D == 128 ? 3 : 4);
-  static constexpr int NR = kQuant ? 2 : 0;
-  static constexpr int kSlots = kQuant ? 4 : 8;  // >= NK + 3: a slot is rewritten only after its tile's softmax
+  static constexpr int NK = kQuant ? 2 : (D == 128 ? 2 : 4);
+  static constexpr int NV = kQuant ? 2 : (D == 128 ? 3 : 4);
+  static constexpr int NR = kQuant ? 6 : 0;
+  static constexpr int kSlots = 8;  // >= NK + 3: a slot is rewritten only after its tile's softmax
   static constexpr int kOffK = kQBytes;
   static constexpr int kOffV = kOffK + NK * kOpBytes;
   static constexpr int kOffRaw = kOffV + NV * kOpBytes;
@@ -52,7 +55,7 @@ template <int CT, int D> struct Wide {
   static constexpr int kOffScale = kOffRawScale + NR * 2 * kTileKeys * 4;  // [kSlots] of [3][64] fp32 (K scales, V scales, log2 bounds), 2 x largest and 2 x smallest bound
   static constexpr int kSlotBytes = kQuant ? 3 * kTileKeys * 4 + 16 : 0;
   static constexpr int kOffHdr = kOffScale + kSlots * kSlotBytes;
-  static_assert(kOffHdr + 1024 <= kWideSmem, "a CTA's shared memory");
+  static_assert(kOffHdr + 1024 <= kSmem, "a CTA's shared memory");
 };
 
 struct WideMaps {
@@ -129,7 +132,7 @@ NVB200_DEVICE uint32_t swz128(int r, int c) { return static_cast<uint32_t>(r * 1
 // r keys 32-63, as if they were two shares of the keys; the tile's products cost what they cost for 128 rows, but a softmax
 // thread has half the work.
 template <int CT, int D, int REP>
-__global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
+__global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
     cache_attention_wide_kernel(const __grid_constant__ WideParams wp, const __grid_constant__ WideMaps maps) {
   using W = Wide<CT, D>;
   using C = CacheType<CT>;
@@ -143,19 +146,23 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, 2)
   const int T = total_work(p, kTileKeys, kUnitRows);  // by every warp
   const int G = active_ctas(T, gridDim.x, kMinTiles);
   zero_uncovered_rows(p, D, kTileKeys, kUnitRows, blockIdx.x, gridDim.x, tid, W::kThreads);
-  if (T == 0 || static_cast<int>(blockIdx.x) >= G) return;
-  const int u0 = range_start(blockIdx.x, T, G), u1 = range_start(blockIdx.x + 1, T, G);
-  Segment seg = find_segment(p, u0, u1, kTileKeys, kUnitRows);
+  const bool work = T > 0 && static_cast<int>(blockIdx.x) < G;
+  const int u0 = work ? range_start(blockIdx.x, T, G) : 0, u1 = work ? range_start(blockIdx.x + 1, T, G) : 0;
+  Segment seg;
+  seg.n = 0;
+  if (work) seg = find_segment(p, u0, u1, kTileKeys, kUnitRows);
+  if (tid == 0) write_cut(p, blockIdx.x, seg, T, G);
+  if (!work) return;
   auto next = [&]() { next_segment(seg, p, u1, kTileKeys, kUnitRows); };
 
   const uint32_t hdr = base + W::kOffHdr;
   const uint32_t b_kfull = hdr, b_kempty = hdr + 32, b_vfull = hdr + 64, b_vempty = hdr + 96;  // up to 4 each
   const uint32_t b_sfull = hdr + 128, b_pready = hdr + 144, b_q = hdr + 168, b_meet = hdr + 176;
   const uint32_t b_pv = hdr + 184;  // 2, like b_sfull and b_pready by tile parity: the softmax may be two P V ahead of one
-  const uint32_t b_rfull = hdr + 240, b_rempty = hdr + 272;              // up to 4 each
-  const uint32_t live_slot = hdr + 304, raw_live = hdr + 368;            // 64-bit words: up to 8, up to 4
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + W::kOffHdr + 400);
-  const uint32_t failed = hdr + 404, dirty = hdr + 408;  // flags
+  const uint32_t b_rfull = hdr + 200, b_rempty = hdr + 264;              // up to 8 each
+  const uint32_t live_slot = hdr + 328, raw_live = hdr + 392;            // 64-bit words: up to 8 each
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + W::kOffHdr + 456);
+  const uint32_t failed = hdr + 460, dirty = hdr + 464;  // flags
 
   if (tid == 0) {
     for (int i = 0; i < W::NK; ++i) mbar_init(b_kfull + 8 * i, W::kQuant ? W::kConvWarps : 1), mbar_init(b_kempty + 8 * i, 1);
@@ -866,10 +873,10 @@ bool make_cache_map(CUtensorMap *map, const void *base, const CacheAttnParams &p
 int wide_rows(const CacheAttnParams &p) { return p.rows <= 64 ? 64 : 128; }  // of a unit
 
 // CTAs: as many as run at once, fewer where the longest possible sequences could not feed them.
-int wide_grid(const CacheAttnParams &p) {
+int wide_grid(const CacheAttnParams &p, int ct) {
   const int64_t units = static_cast<int64_t>(p.batch) * p.hkv * ((p.rows + wide_rows(p) - 1) / wide_rows(p));
   const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.block_size + kTileKeys - 1) / kTileKeys;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * sm_count(), std::max(units, units * tiles / kMinTiles))));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((ct == kE4M3 || ct == kI8 ? 1 : 2) * sm_count(), std::max(units, units * tiles / kMinTiles))));
 }
 
 template <int CT, int D, int REP> int launch_wide(const WideParams &wp, const WideMaps &maps, cudaStream_t s) {
@@ -878,17 +885,17 @@ template <int CT, int D, int REP> int launch_wide(const WideParams &wp, const Wi
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NVB200_ERR_CUDA;
   if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
     if (cudaFuncSetAttribute(cache_attention_wide_kernel<CT, D, REP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kWideSmem) != cudaSuccess) {
+                             Wide<CT, D>::kSmem) != cudaSuccess) {
       cudaGetLastError();
       return NVB200_ERR_CUDA;
     }
     ready.fetch_or(uint64_t{1} << dev, std::memory_order_release);
   }
-  const int grid = wide_grid(wp.a);
-  if (int rc = launch_ex(cache_attention_wide_kernel<CT, D, REP>, dim3(grid), dim3(Wide<CT, D>::kThreads), kWideSmem, s, 1,
+  const int grid = wide_grid(wp.a, CT);
+  if (int rc = launch_ex(cache_attention_wide_kernel<CT, D, REP>, dim3(grid), dim3(Wide<CT, D>::kThreads), Wide<CT, D>::kSmem, s, 1,
                          false, wp, maps))
     return rc;
-  return launch_cache_attention_merge(wp.a, CT, D, kTileKeys, kTileRows / REP, kMinTiles, grid, s);
+  return launch_cache_attention_merge(wp.a, CT, D, kTileRows / REP, grid, s);
 }
 
 template <int CT, int D> int launch_rep(const WideParams &wp, const WideMaps &maps, cudaStream_t s) {
@@ -907,12 +914,13 @@ bool wide_takes(const CacheAttnParams &p) {
   return units <= INT32_MAX / std::max<int64_t>(tiles, 1);
 }
 
-int64_t wide_workspace_bytes(const CacheAttnParams &p, int head_dim) {
-  return 2ll * wide_grid(p) * wide_rows(p) * (head_dim + 4) * 4;
+int64_t wide_workspace_bytes(const CacheAttnParams &p, int ct, int head_dim) {
+  return even_share_bytes(wide_grid(p, ct), wide_rows(p), head_dim);
 }
 
-int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, cudaStream_t stream) {
+int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, void *workspace, cudaStream_t stream) {
   WideParams wp{p, 64, p.scale_log2 < 0.f ? -1.f : 1.f};
+  place_workspace(wp.a, workspace, wide_grid(p, ct));
   while (p.block_size % wp.box_rows != 0) wp.box_rows /= 2;
   wp.a.scale_log2 = std::fabs(p.scale_log2);
   WideMaps maps;
