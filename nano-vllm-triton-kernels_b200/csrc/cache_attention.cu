@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "cache_attention.cuh"
 
@@ -72,13 +73,10 @@ template <int CT, int D, int NT> struct Geometry {
   static constexpr int kStageBytes = 2 * kKvBytes + kScaleBytes + 128;  // a multiple of 128
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kStride = D + 4;  // floats per record: o[D], m, l, M, flag
-  static constexpr int kRecs = NT == 4 ? 2 : kWarps;  // warps' records in shared memory at once
-  static constexpr int kRecords = kRecs * kRows * kStride * 4;
-  // 32 rows: the query fragments (and the rows' factors) do not fit the registers beside the output and live in shared memory,
-  // [D / 16][2][32 lanes] of 16 bytes, as the lanes take them.
-  static constexpr int kQBytes = NT == 4 ? D / 16 * 2 * 32 * 16 + kRows * 4 : 0;
+  static constexpr int kRecords = kWarps * kRows * kStride * 4;
   static constexpr int kPartials = (kMaxSplits + kRows - 1) * kStride * 4;  // splits * ceil(kRows / splits) records
-  static constexpr int kSmem = kRing + kRecords + kQBytes;
+  static constexpr int kRowBytesOut = kRows * 16;  // merged m, l, M, flag per row
+  static constexpr int kSmem = kRing + kRecords + kRowBytesOut;
   static_assert(kPartials <= kRing, "a cluster's records take the ring's place");
   static constexpr int kCtasPerSm = 228 * 1024 / (kSmem + 1024) >= 3 ? 3 : 2;
   // Physical 16-byte chunk of logical chunk c of row r: the 8 rows of an 8 x 16-byte matrix at one logical chunk fall
@@ -107,7 +105,6 @@ template <int D, int NT> struct QueryFrags {
   uint32_t b[D / 16][NT][2];
   float rs[NT][2];
 };
-template <int D> struct QueryFrags<D, 4> {};  // in shared memory
 
 // Replaces every infinity and NaN of the V tile by zero; true if there were any (in any lane).
 template <int CT, int D, int NT> NVB200_DEVICE bool clean_v_tile(uint32_t kt, int lane) {
@@ -132,8 +129,7 @@ template <int CT, int D, int NT> NVB200_DEVICE bool clean_v_tile(uint32_t kt, in
 // Folds one tile. kt: the stage's base address. see[n][e]: which of the tile's keys that row sees, where `edge`; elsewhere
 // every row sees every key.
 template <int CT, int D, int NT>
-NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<D, NT> &q, const uint4 *qs,
-                             const float *rs_s, int lane, bool edge, const uint32_t (&see)[NT][2]) {
+NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<D, NT> &q, int lane, bool edge, const uint32_t (&see)[NT][2]) {
   using G = Geometry<CT, D, NT>;
   using C = CacheType<CT>;
   constexpr int KB = G::kTile / 16;  // 16-key blocks
@@ -144,29 +140,16 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[kb][n][0] = s[kb][n][1] = s[kb][n][2] = s[kb][n][3] = 0.f;
   }
-  // Query fragments of k-step ks.
-  uint32_t qk[NT][2];
-  auto load_q = [&](int ks) {
-    if constexpr (NT == 4) {
-      const uint4 x = qs[(2 * ks) * 32 + lane], y = qs[(2 * ks + 1) * 32 + lane];
-      qk[0][0] = x.x, qk[0][1] = x.y, qk[1][0] = x.z, qk[1][1] = x.w;
-      qk[2][0] = y.x, qk[2][1] = y.y, qk[3][0] = y.z, qk[3][1] = y.w;
-    } else {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) qk[n][0] = q.b[ks][n][0], qk[n][1] = q.b[ks][n][1];
-    }
-  };
   if constexpr (!C::kQuant) {
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      load_q(ks);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const int key = kb * 16 + (mq & 1) * 8 + rr;
         uint32_t a[4];
         ldsm_x4(kt + key * G::kRowBytes + G::chunk(key, 2 * ks + (mq >> 1)) * 16, a);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_ct<CT>(s[kb][n], a, qk[n][0], qk[n][1]);
+        for (int n = 0; n < NT; ++n) mma_ct<CT>(s[kb][n], a, q.b[ks][n][0], q.b[ks][n][1]);
       }
     }
   } else {
@@ -182,14 +165,13 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        load_q(2 * k2 + i);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           uint32_t a[4];
           codes_to_f16<CT>(w[kb][2 * i], a[0], a[2]);
           codes_to_f16<CT>(w[kb][2 * i + 1], a[1], a[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_ct<CT>(s[kb][n], a, qk[n][0], qk[n][1]);
+          for (int n = 0; n < NT; ++n) mma_ct<CT>(s[kb][n], a, q.b[2 * k2 + i][n][0], q.b[2 * k2 + i][n][1]);
         }
       }
     }
@@ -214,10 +196,7 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float &x = s[kb][n][2 * i + e];
-          float f;
-          if constexpr (NT == 4) f = rs_s[8 * n + 2 * (lane & 3) + e];
-          else f = q.rs[n][e];
-          x = C::kQuant ? x * f * ks : x * f;
+          x = C::kQuant ? x * q.rs[n][e] * ks : x * q.rs[n][e];
           if (edge && !((see[n][e] >> key) & 1u)) x = -INFINITY;
         }
       }
@@ -322,9 +301,8 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t wring = smem_addr(smem) + warp * (G::kStages * G::kStageBytes);
-  float *rec = reinterpret_cast<float *>(smem + G::kRing);  // [kRecs][kRows][kStride]
-  uint4 *qs = reinterpret_cast<uint4 *>(smem + G::kRing + G::kRecords);
-  float *rs_s = reinterpret_cast<float *>(qs + D / 16 * 2 * 32);
+  float *rec = reinterpret_cast<float *>(smem + G::kRing);  // [kWarps][kRows][kStride]
+  float4 *row_s = reinterpret_cast<float4 *>(smem + G::kRing + G::kRecords);  // [kRows]
 
   Segment seg;
   int u1, T = 0, ctas = 0;
@@ -418,22 +396,32 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
     cp_async_commit();
   }
 
-  struct Merged { float o, m, l, M, flag; };
-  // Merges `count` records, `stride` floats apart, of one row at column d.
-  auto merge = [&](const float *r, int count, int stride, int d) {
-    Merged x{0.f, -INFINITY, 0.f, -INFINITY, 0.f};
-    for (int k = 0; k < count; ++k) {
-      x.m = fmaxf(x.m, r[k * stride + D]);
-      x.M = fmaxf(x.M, r[k * stride + D + 2]);
+  // Merges `count` records, `stride` floats apart, of the rows [0, rows): first, a thread per row, each record's m becomes
+  // what its o is multiplied by and row_s gets the row's m, l, M, flag; then anybody sums four columns with row4().
+  auto merge_rows = [&](float *r, int rows, int row_stride, int count, int stride) {
+    if (tid < rows) {
+      float *w = r + tid * row_stride + D;
+      float m = -INFINITY, M = -INFINITY, l = 0.f, flag = 0.f;
+      for (int k = 0; k < count; ++k) m = fmaxf(m, w[k * stride]), M = fmaxf(M, w[k * stride + 2]);
+      const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
+      for (int k = 0; k < count; ++k) {
+        float4 *x = reinterpret_cast<float4 *>(w + k * stride);
+        const float4 y = *x;
+        l = fmaf(exp2f(y.x - mu), y.y, l), flag = fmaxf(flag, y.w);
+        x->x = exp2f(y.z - Mu);
+      }
+      row_s[tid] = make_float4(m, l, M, flag);
     }
-    const float mu = x.m == -INFINITY ? 0.f : x.m, Mu = x.M == -INFINITY ? 0.f : x.M;
+    __syncthreads();
+  };
+  auto row4 = [&](const float *row, int d, int count, int stride) {
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < count; ++k) {
-      const float *w = r + k * stride;
-      x.o = fmaf(exp2f(w[D + 2] - Mu), w[d], x.o);
-      x.l = fmaf(exp2f(w[D] - mu), w[D + 1], x.l);
-      x.flag = fmaxf(x.flag, w[D + 3]);
+      const float f = row[k * stride + D];
+      const float4 o = *reinterpret_cast<const float4 *>(row + k * stride + d);
+      y.x = fmaf(f, o.x, y.x), y.y = fmaf(f, o.y, y.y), y.z = fmaf(f, o.z, y.z), y.w = fmaf(f, o.w, y.w);
     }
-    return x;
+    return y;
   };
 
   int stage = 0;  // of the tile to fold next
@@ -448,8 +436,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
     // what the scores of rows 2 t and 2 t + 1 are multiplied by.
     QueryFrags<D, NT> q;
 #pragma unroll
-    for (int n0 = 0; n0 < (NT == 4 ? 1 : NT); ++n0) {
-      const int n = NT == 4 ? warp : n0;  // 32 rows: each warp brings one row tile
+    for (int n = 0; n < NT; ++n) {
       const int r = row0 + 8 * n + g, qi = r / p.group;
       const uint16_t *row = r < p.rows ? static_cast<const uint16_t *>(p.q) + b * p.q_batch_stride +
                                              qi * p.q_token_stride +
@@ -495,19 +482,10 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
           }
         }
       }
-      if constexpr (NT == 4) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          *reinterpret_cast<uint2 *>(reinterpret_cast<uint8_t *>(qs + (2 * ks + (n >> 1)) * 32 + lane) + (n & 1) * 8) =
-              make_uint2(w[ks][0], w[ks][1]);
-        if (t == 0) rs_s[8 * n + g] = f;
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) q.b[ks][n0][0] = w[ks][0], q.b[ks][n0][1] = w[ks][1];
-        q.rs[n0][0] = __shfl_sync(0xffffffffu, f, 8 * t), q.rs[n0][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-      }
+      for (int ks = 0; ks < D / 16; ++ks) q.b[ks][n][0] = w[ks][0], q.b[ks][n][1] = w[ks][1];
+      q.rs[n][0] = __shfl_sync(0xffffffffu, f, 8 * t), q.rs[n][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
     }
-    if constexpr (NT == 4) __syncthreads();
     RowState<D, NT> st;
     st.reset();
 
@@ -563,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
           if (j0 + G::kTile > open && (p.mask ? drafts > 0 : drafts > 1)) dirty |= clean_v_tile<CT, D, NT>(kt, lane);
         }
       }
-      fold_tile<CT, D, NT>(st, kt, q, qs, rs_s, lane, edge, see);
+      fold_tile<CT, D, NT>(st, kt, q, lane, edge, see);
     }
 
     // The warp's record: o, m, l, M, flag per row.
@@ -576,78 +554,56 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
         if constexpr (!C::kQuant) st.M[n][e] = st.m[n][e];
       }
     }
-    auto put_record = [&](int at) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float *w = rec + (at * G::kRows + 8 * n + 2 * t + e) * G::kStride;
+      for (int e = 0; e < 2; ++e) {
+        float *w = rec + (warp * G::kRows + 8 * n + 2 * t + e) * G::kStride;
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            if constexpr (C::kQuant) {
-              *reinterpret_cast<float2 *>(w + 16 * c + 2 * g) = make_float2(st.o[c][n][e], st.o[c][n][2 + e]);
-            } else {
-              w[16 * c + g] = st.o[c][n][e], w[16 * c + 8 + g] = st.o[c][n][2 + e];
-            }
-          }
-          if (g == 0)
-            *reinterpret_cast<float4 *>(w + D) = make_float4(st.m[n][e], st.l[n][e], st.M[n][e], dirty ? 1.f : 0.f);
-        }
-      }
-    };
-    if constexpr (NT == 4) {
-      // Room for two records: warps 2 and 3 hand theirs to warps 0 and 1.
-      if (warp >= 2) put_record(warp - 2);
-      __syncthreads();
-      if (warp < 2) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float *w = rec + (warp * G::kRows + 8 * n + 2 * t + e) * G::kStride;
-            const float4 x = *reinterpret_cast<const float4 *>(w + D);
-            const float mx = fmaxf(st.m[n][e], x.x), Mx = fmaxf(st.M[n][e], x.z);
-            const float mu = mx == -INFINITY ? 0.f : mx, Mu = Mx == -INFINITY ? 0.f : Mx;
-            const float mine = exp2f(st.M[n][e] - Mu), theirs = exp2f(x.z - Mu);
-            st.l[n][e] = st.l[n][e] * exp2f(st.m[n][e] - mu) + x.y * exp2f(x.x - mu);
-            st.m[n][e] = mx, st.M[n][e] = Mx;
-            dirty |= x.w != 0.f;
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              const float a0 = C::kQuant ? w[16 * c + 2 * g] : w[16 * c + g];
-              const float a1 = C::kQuant ? w[16 * c + 2 * g + 1] : w[16 * c + 8 + g];
-              st.o[c][n][e] = fmaf(a0, theirs, st.o[c][n][e] * mine);
-              st.o[c][n][2 + e] = fmaf(a1, theirs, st.o[c][n][2 + e] * mine);
-            }
+        for (int c = 0; c < D / 16; ++c) {
+          if constexpr (C::kQuant) {
+            *reinterpret_cast<float2 *>(w + 16 * c + 2 * g) = make_float2(st.o[c][n][e], st.o[c][n][2 + e]);
+          } else {
+            w[16 * c + g] = st.o[c][n][e], w[16 * c + 8 + g] = st.o[c][n][2 + e];
           }
         }
-        __syncwarp();
-        put_record(warp);
+        if (g == 0) *reinterpret_cast<float4 *>(w + D) = make_float4(st.m[n][e], st.l[n][e], st.M[n][e], dirty ? 1.f : 0.f);
       }
-    } else {
-      put_record(warp);
     }
     __syncthreads();
 
     const int32_t *bt = p.block_table ? p.block_table + b * p.bt_stride : nullptr;
     const int nrows = min(G::kRows, p.rows - row0);
-    auto write = [&](int r, int d, const Merged &x) {  // r: row within the unit
+    constexpr int kPer = D / 4;  // threads per row
+    auto write = [&](int r, int d, const float4 &o, const float4 &x) {  // r: row within the unit; x: its m, l, M, flag
       const int row = row0 + r, qi = row / p.group, gq = row - qi * p.group;
-      float y = 0.f;
-      if (qi < drafts) {
-        // l > 0 wherever a key was seen; NaN (a NaN score) is passed on.
-        if (x.l != 0.f) y = x.o / x.l * (C::kQuant ? exp2f(x.M - x.m) : 1.f);
-        if (CT != kI8 && x.flag != 0.f) y = add_nonfinite<CT>(p, bt, b, h, qi, d, ctx, L, drafts, y);
+      float y[4] = {o.x, o.y, o.z, o.w};
+      // l > 0 wherever a key was seen; NaN (a NaN score) is passed on.
+      const float f = x.y == 0.f ? 0.f : (C::kQuant ? exp2f(x.z - x.x) : 1.f) / x.y;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        y[k] = qi < drafts && x.y != 0.f ? y[k] * f : 0.f;
+        if (CT != kI8 && x.w != 0.f && qi < drafts) y[k] = add_nonfinite<CT>(p, bt, b, h, qi, d + k, ctx, L, drafts, y[k]);
       }
-      const int64_t idx = ((static_cast<int64_t>(b) * p.n + qi) * p.hq + h * p.group + gq) * D + d;
-      if (C::kQuant ? p.q_is_f16 : CT == kF16) static_cast<__half *>(p.out)[idx] = __float2half_rn(y);
-      else static_cast<__nv_bfloat16 *>(p.out)[idx] = __float2bfloat16_rn(y);
+      const bool f16 = C::kQuant ? p.q_is_f16 : CT == kF16;
+      const uint32_t lo = f16 ? pack_f16x2(y[0], y[1]) : pack_bf16x2(y[0], y[1]);
+      const uint32_t hi = f16 ? pack_f16x2(y[2], y[3]) : pack_bf16x2(y[2], y[3]);
+      uint16_t *to = static_cast<uint16_t *>(p.out) + ((static_cast<int64_t>(b) * p.n + qi) * p.hq + h * p.group + gq) * D + d;
+      if ((reinterpret_cast<uintptr_t>(p.out) & 7) == 0) {
+        *reinterpret_cast<uint2 *>(to) = make_uint2(lo, hi);
+      } else {
+        to[0] = static_cast<uint16_t>(lo), to[1] = static_cast<uint16_t>(lo >> 16);
+        to[2] = static_cast<uint16_t>(hi), to[3] = static_cast<uint16_t>(hi >> 16);
+      }
     };
+    merge_rows(rec, nrows, G::kStride, kWarps, G::kRows * G::kStride);
 
     if constexpr (CLUSTER) {
       if (p.splits == 1) {
-        for (int e = tid; e < nrows * D; e += kThreads)
-          write(e / D, e % D, merge(rec + e / D * G::kStride, G::kRecs, G::kRows * G::kStride, e % D));
+        for (int e = tid; e < nrows * kPer; e += kThreads) {
+          const int r = e / kPer, d = e % kPer * 4;
+          write(r, d, row4(rec + r * G::kStride, d, kWarps, G::kRows * G::kStride), row_s[r]);
+        }
         return;
       }
       // Row r is finished by CTA r mod splits: every CTA sends its merged record there, into the ring's place (the first
@@ -657,34 +613,33 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
       cp_async_wait<0>();
       cluster_arrive();
       cluster_wait();
-      for (int e = tid; e < nrows * D; e += kThreads) {
-        const int r = e / D, d = e - r * D;
-        const Merged x = merge(rec + r * G::kStride, G::kRecs, G::kRows * G::kStride, d);
+      for (int e = tid; e < nrows * kPer; e += kThreads) {
+        const int r = e / kPer, d = e % kPer * 4;
+        const float4 o = row4(rec + r * G::kStride, d, kWarps, G::kRows * G::kStride);
         const uint32_t to = map_shared_to(smem_addr(part + ((r / p.splits) * p.splits + rank) * G::kStride), r % p.splits);
-        st_cluster_f32(to + d * 4, x.o);
-        if (d == 0) {
-          st_cluster_f32(to + D * 4, x.m), st_cluster_f32(to + (D + 1) * 4, x.l);
-          st_cluster_f32(to + (D + 2) * 4, x.M), st_cluster_f32(to + (D + 3) * 4, x.flag);
-        }
+        st_cluster_v4(to + d * 4, o);
+        if (d == 0) st_cluster_v4(to + D * 4, row_s[r]);
       }
       cluster_arrive();
       cluster_wait();
-      for (int e = tid; e < nrows * D; e += kThreads) {
-        const int r = e / D, d = e - r * D;
-        if (r % p.splits == rank) write(r, d, merge(part + (r / p.splits) * p.splits * G::kStride, p.splits, G::kStride, d));
+      const int mine = nrows > rank ? (nrows - rank + p.splits - 1) / p.splits : 0;  // rows rank, rank + splits, ...
+      merge_rows(part, mine, p.splits * G::kStride, p.splits, G::kStride);
+      for (int e = tid; e < mine * kPer; e += kThreads) {
+        const int i = e / kPer, d = e % kPer * 4;
+        write(i * p.splits + rank, d, row4(part + i * p.splits * G::kStride, d, p.splits, G::kStride), row_s[i]);
       }
       return;
     } else {
       const bool whole = seg.n == seg.s.tiles;
       float *out = p.records + static_cast<int64_t>(record_slot(blockIdx.x, seg.unit_u, T, ctas)) * G::kRows * G::kStride;
-      for (int e = tid; e < nrows * D; e += kThreads) {
-        const int r = e / D, d = e - r * D;
-        const Merged x = merge(rec + r * G::kStride, G::kRecs, G::kRows * G::kStride, d);
+      for (int e = tid; e < nrows * kPer; e += kThreads) {
+        const int r = e / kPer, d = e % kPer * 4;
+        const float4 o = row4(rec + r * G::kStride, d, kWarps, G::kRows * G::kStride);
         if (whole) {
-          write(r, d, x);
+          write(r, d, o, row_s[r]);
         } else {
-          out[r * G::kStride + d] = x.o;
-          if (d == 0) *reinterpret_cast<float4 *>(out + r * G::kStride + D) = make_float4(x.m, x.l, x.M, x.flag);
+          *reinterpret_cast<float4 *>(out + r * G::kStride + d) = o;
+          if (d == 0) *reinterpret_cast<float4 *>(out + r * G::kStride + D) = row_s[r];
         }
       }
       next_segment(seg, p, u1, G::kTile, G::kRows);
@@ -709,12 +664,12 @@ template <typename Kernel> int allow_smem(Kernel kernel, int bytes, std::atomic<
   return NVB200_OK;
 }
 
-// Largest power of two of CTAs per cluster that the longest possible sequence feeds with a tile per warp, while the clusters
+// Largest power of two of CTAs per cluster that the longest possible sequence feeds with a tile for every other warp, while the clusters
 // fit on the GPU at once.
 int cluster_splits(const CacheAttnParams &p, int64_t units, int tile, int ctas_per_sm) {
   const int64_t max_keys = static_cast<int64_t>(p.max_pages) * p.block_size;
   int s = 1;
-  while (s < kMaxSplits && 2 * s * units <= static_cast<int64_t>(ctas_per_sm) * sm_count() && 2 * s * kWarps * tile <= max_keys)
+  while (s < kMaxSplits && 2 * s * units <= static_cast<int64_t>(ctas_per_sm) * sm_count() && s * kWarps * tile <= max_keys)
     s *= 2;
   return s;
 }
@@ -727,15 +682,26 @@ template <int CT, int D, int NT> NarrowShape shape_of(const CacheAttnParams &p) 
   using G = Geometry<CT, D, NT>;
   return {static_cast<int64_t>(p.hkv) * ((p.rows + G::kRows - 1) / G::kRows), G::kTile, G::kRows, G::kCtasPerSm};
 }
-NarrowShape narrow_shape(const CacheAttnParams &p, int ct, int d) {
-#define NVB200_SHAPE(CT)                                                                                          (d == 64 ? (p.rows <= 8 ? shape_of<CT, 64, 1>(p) : shape_of<CT, 64, 2>(p))                                               : (p.rows <= 8 ? shape_of<CT, 128, 1>(p) : shape_of<CT, 128, 2>(p)))
+
+// The one place that picks a kernel: f(cache type, head_dim, row tiles of 8) as integral constants. More than 16 rows are
+// blocks of 16 (a form with 32 rows a warp, its queries in shared memory, took 92 us where this takes 73: it has half the
+// warps, and the code is bound by dependent issue).
+template <int I> using Int = std::integral_constant<int, I>;
+template <typename F> auto with_kernel(const CacheAttnParams &p, int ct, int d, F &&f) {
+  auto rows = [&](auto CT, auto D) {
+    if (p.rows <= 8) return f(CT, D, Int<1>{});
+    return f(CT, D, Int<2>{});
+  };
+  auto dim = [&](auto CT) { return d == 64 ? rows(CT, Int<64>{}) : rows(CT, Int<128>{}); };
   switch (ct) {
-    case kBf16: return NVB200_SHAPE(kBf16);
-    case kF16: return NVB200_SHAPE(kF16);
-    case kE4M3: return NVB200_SHAPE(kE4M3);
-    default: return NVB200_SHAPE(kI8);
+    case kBf16: return dim(Int<kBf16>{});
+    case kF16: return dim(Int<kF16>{});
+    case kE4M3: return dim(Int<kE4M3>{});
+    default: return dim(Int<kI8>{});
   }
-#undef NVB200_SHAPE
+}
+NarrowShape narrow_shape(const CacheAttnParams &p, int ct, int d) {
+  return with_kernel(p, ct, d, [&](auto CT, auto D, auto NT) { return shape_of<CT(), D(), NT()>(p); });
 }
 
 int64_t total_tiles(const CacheAttnParams &p, const NarrowShape &n) {
@@ -779,20 +745,17 @@ template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_s
                    dim3(kThreads), G::kSmem, s, p.splits, false, p);
 }
 
-template <int CT> int launch_dim(CacheAttnParams &p, int d, int num_splits, void *workspace, cudaStream_t s) {
-  if (d == 64)
-    return p.rows <= 8    ? launch_narrow<CT, 64, 1>(p, num_splits, workspace, s)
-           : p.rows <= 16 ? launch_narrow<CT, 64, 2>(p, num_splits, workspace, s)
-                          : launch_narrow<CT, 64, 4>(p, num_splits, workspace, s);
-  return p.rows <= 8    ? launch_narrow<CT, 128, 1>(p, num_splits, workspace, s)
-         : p.rows <= 16 ? launch_narrow<CT, 128, 2>(p, num_splits, workspace, s)
-                        : launch_narrow<CT, 128, 4>(p, num_splits, workspace, s);
+// Whether a call takes the wide kernel (128 rows a CTA on the 5th-generation tensor cores) rather than blocks of 16 rows of
+// this one. Measured on B200, head_dim 128, group 4, this kernel against the wide one, us:
+//   16-bit cache, 32 sequences of up to 2048 keys: 64 rows 80 / 87, 128 rows 151 / 99
+//   16-bit cache, 8 sequences of up to 16384 keys: 64 rows 145 / 97, 256 rows 410 / 116
+//   8-bit cache,  32 sequences of up to 2048 keys: 64 rows 74 / 133, 128 rows 132 / 152
+//   8-bit cache,  8 sequences of up to 16384 keys: 64 rows 107 / 146, 256 rows 351 / 228
+// (the wide kernel has to convert 8-bit tiles through shared memory; many keys let its roles run undisturbed).
+bool prefers_wide(const CacheAttnParams &p, int ct) {
+  if (ct == kE4M3 || ct == kI8) return p.rows > 128;
+  return p.rows > 64 || (p.rows > 32 && static_cast<int64_t>(p.max_pages) * p.block_size > 2 * kFewKeys);
 }
-
-#ifndef NVB200_NARROW_ROWS
-#define NVB200_NARROW_ROWS 64
-#endif
-constexpr int kNarrowRows = NVB200_NARROW_ROWS;
 
 // Checks a call and fills `p` (all but the workspace) and *ct; *launch = false where there is nothing to do.
 int prepare_attention(const nvb200_cache_attention_args *a, CacheAttnParams &p, int *ct, bool *launch) {
@@ -855,7 +818,7 @@ extern "C" int64_t nvb200_cache_attention_workspace_size(const nvb200_cache_atte
   bool launch = false;
   if (prepare_attention(a, p, &ct, &launch) != NVB200_OK) return -1;
   if (!launch) return 0;
-  if (p.rows > kNarrowRows && a->num_splits == 0 && wide_takes(p)) return wide_workspace_bytes(p, ct, a->head_dim);
+  if (prefers_wide(p, ct) && a->num_splits == 0 && wide_takes(p, ct)) return wide_workspace_bytes(p, ct, a->head_dim);
   const NarrowShape n = narrow_shape(p, ct, a->head_dim);
   return even_share_bytes(narrow_grid(p, n, a->num_splits), n.rows, a->head_dim);
 }
@@ -873,15 +836,12 @@ extern "C" int nvb200_cache_attention(const nvb200_cache_attention_args *a, void
   if (workspace && workspace_bytes < need) return NVB200_ERR_ARG;
   if (need == 0) workspace = nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (p.rows > kNarrowRows && a->num_splits == 0 && workspace && wide_takes(p)) {
+  if (prefers_wide(p, ct) && a->num_splits == 0 && workspace && wide_takes(p, ct)) {
     const int rc = launch_cache_attention_wide(p, ct, a->head_dim, workspace, s);
     if (rc != NVB200_ERR_UNSUPPORTED) return rc;
     workspace = nullptr;  // sized for the other kernel: the cluster form needs none
   }
-  switch (ct) {
-    case kBf16: return launch_dim<kBf16>(p, a->head_dim, a->num_splits, workspace, s);
-    case kF16: return launch_dim<kF16>(p, a->head_dim, a->num_splits, workspace, s);
-    case kE4M3: return launch_dim<kE4M3>(p, a->head_dim, a->num_splits, workspace, s);
-    default: return launch_dim<kI8>(p, a->head_dim, a->num_splits, workspace, s);
-  }
+  return with_kernel(p, ct, a->head_dim, [&](auto CT, auto D, auto NT) {
+    return launch_narrow<CT(), D(), NT()>(p, a->num_splits, workspace, s);
+  });
 }

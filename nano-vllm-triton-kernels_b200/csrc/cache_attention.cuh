@@ -69,8 +69,9 @@ NVB200_DEVICE uint32_t map_shared_to(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-NVB200_DEVICE void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+NVB200_DEVICE void st_cluster_v4(uint32_t addr, const float4 &v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
 }
 NVB200_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 NVB200_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -294,7 +295,7 @@ NVB200_DEVICE float add_nonfinite(const CacheAttnParams &p, const int32_t *bt, i
 
 // The wide kernel (cache_attention_wide.cu). NVB200_ERR_UNSUPPORTED where it does not take the call (pages whose size is
 // not a multiple of 8 tokens, cache strides that no tensor map describes).
-bool wide_takes(const CacheAttnParams &p);
+bool wide_takes(const CacheAttnParams &p, int ct);
 int64_t wide_workspace_bytes(const CacheAttnParams &p, int ct, int head_dim);
 int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, void *workspace, cudaStream_t stream);
 

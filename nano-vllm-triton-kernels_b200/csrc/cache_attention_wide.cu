@@ -870,11 +870,12 @@ bool make_cache_map(CUtensorMap *map, const void *base, const CacheAttnParams &p
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int wide_rows(const CacheAttnParams &p) { return p.rows <= 64 ? 64 : 128; }  // of a unit
+// Rows of a unit. 8-bit caches come with more than 128 rows only.
+int wide_rows(const CacheAttnParams &p, int ct) { return p.rows <= 64 && ct != kE4M3 && ct != kI8 ? 64 : 128; }
 
 // CTAs: as many as run at once, fewer where the longest possible sequences could not feed them.
 int wide_grid(const CacheAttnParams &p, int ct) {
-  const int64_t units = static_cast<int64_t>(p.batch) * p.hkv * ((p.rows + wide_rows(p) - 1) / wide_rows(p));
+  const int64_t units = static_cast<int64_t>(p.batch) * p.hkv * ((p.rows + wide_rows(p, ct) - 1) / wide_rows(p, ct));
   const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.block_size + kTileKeys - 1) / kTileKeys;
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((ct == kE4M3 || ct == kI8 ? 1 : 2) * sm_count(), std::max(units, units * tiles / kMinTiles))));
 }
@@ -899,23 +900,26 @@ template <int CT, int D, int REP> int launch_wide(const WideParams &wp, const Wi
 }
 
 template <int CT, int D> int launch_rep(const WideParams &wp, const WideMaps &maps, cudaStream_t s) {
-  return wide_rows(wp.a) == 64 ? launch_wide<CT, D, 2>(wp, maps, s) : launch_wide<CT, D, 1>(wp, maps, s);
+  if constexpr (!CacheType<CT>::kQuant) {
+    if (wide_rows(wp.a, CT) == 64) return launch_wide<CT, D, 2>(wp, maps, s);
+  }
+  return launch_wide<CT, D, 1>(wp, maps, s);
 }
 
 }  // namespace
 
-bool wide_takes(const CacheAttnParams &p) {
+bool wide_takes(const CacheAttnParams &p, int ct) {
   // Boxes are runs of tokens of one page: 8 rows is the swizzle's period. A zero scale would make masked scores 0 * -inf.
   if (p.block_size % 8 != 0 || p.num_blocks > INT32_MAX || !aligned16(p.out) || !(std::fabs(p.scale_log2) > 1e-30f))
     return false;
   // Tiles are counted in 32 bits.
   const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.block_size + kTileKeys - 1) / kTileKeys;
-  const int64_t units = static_cast<int64_t>(p.hkv) * ((p.rows + wide_rows(p) - 1) / wide_rows(p)) * p.batch;
+  const int64_t units = static_cast<int64_t>(p.hkv) * ((p.rows + wide_rows(p, ct) - 1) / wide_rows(p, ct)) * p.batch;
   return units <= INT32_MAX / std::max<int64_t>(tiles, 1);
 }
 
 int64_t wide_workspace_bytes(const CacheAttnParams &p, int ct, int head_dim) {
-  return even_share_bytes(wide_grid(p, ct), wide_rows(p), head_dim);
+  return even_share_bytes(wide_grid(p, ct), wide_rows(p, ct), head_dim);
 }
 
 int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, void *workspace, cudaStream_t stream) {
