@@ -5,9 +5,10 @@
 // the writes, 4 bytes per row either way, are merged in the L2. kv_quant_math.cuh has the quantiser.
 //
 // All three are HBM-bound: every row is read once and written once, and a row's maximum is taken from registers, so
-// nothing is read a second time. A group of D / 8 lanes (a power of two of them) holds a row, 8 elements a lane: 16-byte
-// loads of 16-bit inputs, 8-byte stores of codes, and the maximum by shuffles within the group.
+// nothing is read a second time. A group of D / 16 lanes (a power of two of them) holds a row, 8 elements of each half a
+// lane: 16-byte loads of 16-bit inputs, 8-byte stores of codes, and the maximum by shuffles within the group.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv_quant_math.cuh"
@@ -18,6 +19,24 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 
+// Division of 32-bit numbers by a divisor that the host knows (Granlund and Montgomery, "Division by invariant integers
+// using multiplication", 1994, figure 4.1).
+struct Divider {
+  uint32_t d, m;
+  uint8_t s1, s2;
+  void set(uint32_t divisor) {
+    int l = 0;
+    while ((uint64_t{1} << l) < divisor) ++l;
+    d = divisor;
+    m = static_cast<uint32_t>((((uint64_t{1} << l) - divisor) << 32) / divisor + 1);
+    s1 = l > 0, s2 = l > 0 ? l - 1 : 0;
+  }
+  NVB200_DEVICE uint32_t quotient(uint32_t n) const {
+    const uint32_t t = __umulhi(m, n);
+    return (t + ((n - t) >> s1)) >> s2;
+  }
+};
+
 struct QuantCache {
   uint8_t *k;
   uint8_t *v;
@@ -27,12 +46,13 @@ struct QuantCache {
   int block_size;
   int hkv;
   int d;
+  Divider by_block, by_hkv;  // by block_size, by hkv
   int32_t *status;
 };
 
 // Index in the scale arrays of head h of slot s.
 NVB200_DEVICE int64_t scale_index(const QuantCache &c, int64_t slot, int h) {
-  const uint32_t blk = static_cast<uint32_t>(slot) / static_cast<uint32_t>(c.block_size);  // num_slots < 2^32
+  const uint32_t blk = c.by_block.quotient(static_cast<uint32_t>(slot));  // num_slots < 2^32
   const uint32_t in = static_cast<uint32_t>(slot) - blk * static_cast<uint32_t>(c.block_size);
   return (static_cast<int64_t>(blk) * c.hkv + h) * c.block_size + in;
 }
@@ -53,23 +73,76 @@ NVB200_DEVICE int64_t load_slot(const void *slots, int slot64, int64_t t) {
                 : static_cast<int64_t>(__ldg(static_cast<const int *>(slots) + t));
 }
 
-// Eight consecutive elements as fp32. p is 16-byte aligned.
-template <typename T> NVB200_DEVICE void load8(const T *p, float (&f)[8]);
-template <> NVB200_DEVICE void load8<__nv_bfloat16>(const __nv_bfloat16 *p, float (&f)[8]) {
-  unpack8(__ldg(reinterpret_cast<const uint4 *>(p)), f);
-}
-template <> NVB200_DEVICE void load8<__half>(const __half *p, float (&f)[8]) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// What a lane holds of a row: elements [8 j, 8 j + 8) and [D / 2 + 8 j, D / 2 + 8 j + 8), as they were loaded.
+template <typename T> struct Piece {
+  static constexpr int kWords = sizeof(T) / 2;  // 16-byte words of 8 elements
+  uint4 w[2 * kWords];
+  NVB200_DEVICE void clear() {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-    f[2 * i] = x.x, f[2 * i + 1] = x.y;
+    for (int i = 0; i < 2 * kWords; ++i) w[i] = make_uint4(0, 0, 0, 0);
   }
+  NVB200_DEVICE void load(const T *p, int half) {  // p + 8 j; 16-byte aligned, as is half * sizeof(T)
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+      w[kWords + i] = __ldg(reinterpret_cast<const uint4 *>(p + half) + i);
+    }
+  }
+  NVB200_DEVICE void values(int h, float (&f)[8]) const {
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 u = w[2 * h + i];
+        f[4 * i] = __uint_as_float(u.x), f[4 * i + 1] = __uint_as_float(u.y);
+        f[4 * i + 2] = __uint_as_float(u.z), f[4 * i + 3] = __uint_as_float(u.w);
+      }
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const uint32_t x[4] = {w[h].x, w[h].y, w[h].z, w[h].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&x[i]));
+        f[2 * i] = y.x, f[2 * i + 1] = y.y;
+      }
+    } else {
+      unpack8(w[h], f);
+    }
+  }
+  // The largest magnitude's bits, in the element's own type (infinities and NaNs are above every finite value).
+  NVB200_DEVICE uint32_t amax() const {
+    uint32_t m = 0;
+    constexpr uint32_t kAbs = std::is_same<T, float>::value ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+#pragma unroll
+    for (int i = 0; i < 2 * kWords; ++i) {
+      const uint32_t x[4] = {w[i].x & kAbs, w[i].y & kAbs, w[i].z & kAbs, w[i].w & kAbs};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = std::is_same<T, float>::value ? max(m, x[e]) : __vmaxu2(m, x[e]);
+    }
+    return std::is_same<T, float>::value ? m : max(m & 0xFFFFu, m >> 16);
+  }
+};
+
+// Bits of a non-negative value of type T as those of the fp32 value.
+template <typename T> NVB200_DEVICE uint32_t bits32(uint32_t b) {
+  if constexpr (std::is_same<T, float>::value) return b;
+  else if constexpr (std::is_same<T, __half>::value)
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(b))));
+  else return b << 16;
 }
-template <> NVB200_DEVICE void load8<float>(const float *p, float (&f)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+
+// The largest of ka and of va over a group of LPR lanes, as fp32 bits: one shuffle for both where they have 16 bits.
+template <typename T, int LPR> NVB200_DEVICE void group_amax(uint32_t &ka, uint32_t &va) {
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) {
+      ka = max(ka, __shfl_xor_sync(0xffffffffu, ka, o));
+      va = max(va, __shfl_xor_sync(0xffffffffu, va, o));
+    }
+  } else {
+    uint32_t m = ka | va << 16;
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    ka = bits32<T>(m & 0xFFFFu), va = bits32<T>(m >> 16);
+  }
 }
 
 NVB200_DEVICE uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
@@ -80,53 +153,50 @@ NVB200_DEVICE uint32_t amax8(const float (&f)[8]) {
   return a;
 }
 
-// Row u (token u / hkv, head u % hkv) is held by a group of LPR lanes; lanes at or past D / 8 hold nothing.
+// Row u (token u / hkv, head u % hkv) is held by a group of LPR lanes; lanes at or past D / 16 hold nothing. All loads are
+// in flight at once; the values do not wait for the slot (a token without one has its row read for nothing).
 template <typename T, int FMT, int LPR>
 __global__ void __launch_bounds__(kQuantThreads) store_quant_kernel(const __grid_constant__ StoreQuantArgs a) {
-  const int j = threadIdx.x % LPR;
-  const bool on = 8 * j < a.c.d;
-  const uint32_t step = gridDim.x * (kQuantThreads / LPR);
-  const uint32_t first = blockIdx.x * (kQuantThreads / LPR) + threadIdx.x / LPR;
-  // Every lane of a warp runs the same number of rounds: the shuffles below are over whole warps.
-  for (uint32_t base = first - threadIdx.x % 32 / LPR; base < a.rows; base += step) {
-    const uint32_t u = base + threadIdx.x % 32 / LPR;
-    int64_t slot = -1;
-    uint32_t t = 0, h = 0;
-    if (u < a.rows) {
-      t = u / static_cast<uint32_t>(a.c.hkv), h = u - t * a.c.hkv;
-      slot = load_slot(a.slots, a.slot64, t);
-      if (slot < -1 || slot >= a.c.num_slots) {
-        if (j == 0) set_status(a.c.status, NVB200_STATUS_BAD_SLOT);
-        slot = -1;
-      }
-    }
-    float k[8] = {}, v[8] = {};
-    if (slot >= 0 && on) {
-      load8(reinterpret_cast<const T *>(a.key) + t * a.key_stride + static_cast<int64_t>(h) * a.c.d + 8 * j, k);
-      load8(reinterpret_cast<const T *>(a.value) + t * a.value_stride + static_cast<int64_t>(h) * a.c.d + 8 * j, v);
-    }
-    uint32_t ka = amax8(k), va = amax8(v);
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) {
-      ka = max(ka, __shfl_xor_sync(0xffffffffu, ka, o));
-      va = max(va, __shfl_xor_sync(0xffffffffu, va, o));
-    }
-    if (slot < 0) continue;
-    const RowScale ks = row_scale<FMT>(ka), vs = row_scale<FMT>(va);
+  const int j = threadIdx.x % LPR, half = a.c.d / 2;
+  const bool on = 8 * j < half;
+  const uint32_t u = blockIdx.x * (kQuantThreads / LPR) + threadIdx.x / LPR;
+  const uint32_t t = a.c.by_hkv.quotient(u), h = u - t * a.c.hkv;
+  Piece<T> k, v;
+  k.clear(), v.clear();
+  int64_t slot = -1;
+  if (u < a.rows) {
+    slot = load_slot(a.slots, a.slot64, t);
     if (on) {
-      const int64_t off = (slot * a.c.hkv + h) * a.c.d + 8 * j;
-      *reinterpret_cast<uint2 *>(a.c.k + off) = quantise8<FMT>(k, ks);
-      *reinterpret_cast<uint2 *>(a.c.v + off) = quantise8<FMT>(v, vs);
+      k.load(reinterpret_cast<const T *>(a.key) + t * a.key_stride + static_cast<int64_t>(h) * a.c.d + 8 * j, half);
+      v.load(reinterpret_cast<const T *>(a.value) + t * a.value_stride + static_cast<int64_t>(h) * a.c.d + 8 * j, half);
     }
-    if (j == 0) {
-      const int64_t si = scale_index(a.c, slot, h);
-      a.c.k_scale[si] = ks.scale;
-      a.c.v_scale[si] = vs.scale;
+  }
+  uint32_t ka = k.amax(), va = v.amax();
+  group_amax<T, LPR>(ka, va);
+  if (slot < 0 || slot >= a.c.num_slots) {
+    if (slot != -1 && j == 0) set_status(a.c.status, NVB200_STATUS_BAD_SLOT);
+    return;
+  }
+  const RowScale ks = row_scale<FMT>(ka), vs = row_scale<FMT>(va);
+  if (on) {
+    const int64_t off = (slot * a.c.hkv + h) * a.c.d + 8 * j;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float x[8];
+      k.values(i, x);
+      *reinterpret_cast<uint2 *>(a.c.k + off + i * half) = quantise8<FMT>(x, ks);
+      v.values(i, x);
+      *reinterpret_cast<uint2 *>(a.c.v + off + i * half) = quantise8<FMT>(x, vs);
     }
+  }
+  if (j == 0) {
+    const int64_t si = scale_index(a.c, slot, h);
+    a.c.k_scale[si] = ks.scale;
+    a.c.v_scale[si] = vs.scale;
   }
 }
 
-// Rows that the vector kernel does not take (D not a multiple of 8 or above 256, addresses not 16-byte aligned): one
+// Rows that the vector kernel does not take (D not a multiple of 16 or above 512, addresses not 16-byte aligned): one
 // warp per row, one element per access, the row read twice (the second time from the L1).
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kQuantThreads) store_quant_any_kernel(const __grid_constant__ StoreQuantArgs a) {
@@ -160,18 +230,24 @@ int grid_for(int64_t units, int64_t per_cta, int per_sm) {
       1, std::min<int64_t>((units + per_cta - 1) / per_cta, static_cast<int64_t>(sm_count()) * per_sm)));
 }
 
+// f(lanes that hold a row of D elements, 16 a lane)
+template <typename F> int with_lanes(int d, F &&f) {
+  if (d <= 64) return f(std::integral_constant<int, 4>{});
+  if (d <= 128) return f(std::integral_constant<int, 8>{});
+  return d <= 256 ? f(std::integral_constant<int, 16>{}) : f(std::integral_constant<int, 32>{});
+}
+bool fits_lanes(int d) { return d % 16 == 0 && d <= 512; }
+
 template <typename T, int FMT> int launch_store_quant(const StoreQuantArgs &a, bool vec, cudaStream_t s) {
   if (!vec) {
     store_quant_any_kernel<T, FMT><<<grid_for(2ll * a.rows, kQuantThreads / 32, 8), kQuantThreads, 0, s>>>(a);
     return launch_status();
   }
-  const int lanes = a.c.d / 8;
-  const int lpr = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : 32);
-  const int grid = grid_for(a.rows, kQuantThreads / lpr, 8);
-  if (lpr == 8) store_quant_kernel<T, FMT, 8><<<grid, kQuantThreads, 0, s>>>(a);
-  else if (lpr == 16) store_quant_kernel<T, FMT, 16><<<grid, kQuantThreads, 0, s>>>(a);
-  else store_quant_kernel<T, FMT, 32><<<grid, kQuantThreads, 0, s>>>(a);
-  return launch_status();
+  return with_lanes(a.c.d, [&](auto lanes) {
+    constexpr uint32_t kGroups = kQuantThreads / lanes();
+    store_quant_kernel<T, FMT, lanes()><<<(a.rows + kGroups - 1) / kGroups, kQuantThreads, 0, s>>>(a);
+    return launch_status();
+  });
 }
 
 template <typename T> int launch_store_fmt(const StoreQuantArgs &a, int fmt, bool vec, cudaStream_t s) {
@@ -193,82 +269,98 @@ struct QknrQuantArgs {
   const float *cos_sin;
   int64_t cs_stride, num_positions;
   __nv_bfloat16 *q_out, *k_out;
-  uint32_t units;  // tokens * heads
-  int hq, heads;   // heads = hq + 2 hkv
+  uint32_t units;         // groups of R heads
+  Divider by_parts;       // by a token's groups
+  int hq, heads;          // heads = hq + 2 hkv
   float eps;
   QuantCache c;
 };
 
-template <int D, int FMT>
+template <int D, int FMT, int R>
 __global__ void __launch_bounds__(kQuantThreads) qknr_quant_kernel(const __grid_constant__ QknrQuantArgs a) {
   constexpr int HALF = D / 2, LPH = D / 16;
-  const int j = threadIdx.x % LPH, in_warp = threadIdx.x % 32 / LPH;
-  const uint32_t step = gridDim.x * (kQuantThreads / LPH);
-  for (uint32_t base = blockIdx.x * (kQuantThreads / LPH) + threadIdx.x / 32 * (32 / LPH); base < a.units; base += step) {
-    const uint32_t u = base + in_warp;
-    const bool live = u < a.units;
-    const uint32_t t = live ? u / static_cast<uint32_t>(a.heads) : 0;
-    const int head = live ? static_cast<int>(u - t * a.heads) : 0;
+  const int j = threadIdx.x % LPH;
+  const uint32_t u = blockIdx.x * (kQuantThreads / LPH) + threadIdx.x / LPH;
+  const bool live = u < a.units;
+  const uint32_t t = live ? a.by_parts.quotient(u) : 0;
+  const int head0 = live ? static_cast<int>(u - t * a.by_parts.d) * R : a.heads;
+  uint4 xa[R], xb[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    xa[i] = xb[i] = make_uint4(0, 0, 0, 0);
+    const int head = head0 + i;
+    if (head < a.heads) {
+      const __nv_bfloat16 *x = head < a.hq ? a.q + t * a.q_stride + static_cast<int64_t>(head) * D
+                               : head < a.hq + a.c.hkv
+                                   ? a.k + t * a.k_stride + static_cast<int64_t>(head - a.hq) * D
+                                   : a.v + t * a.v_stride + static_cast<int64_t>(head - a.hq - a.c.hkv) * D;
+      xa[i] = __ldg(reinterpret_cast<const uint4 *>(x + 8 * j));
+      xb[i] = __ldg(reinterpret_cast<const uint4 *>(x + HALF + 8 * j));
+    }
+  }
+  const bool rotates = head0 < a.hq + a.c.hkv;  // a head of this lane's that is q or k
+  int64_t slot = -1, pos = 0;
+  if (live) {
+    if (head0 + R > a.hq) slot = __ldg(a.slots + t);
+    if (rotates) pos = __ldg(a.positions + t);
+  }
+  if (slot < -1 || slot >= a.c.num_slots) {
+    if (j == 0) set_status(a.c.status, NVB200_STATUS_BAD_SLOT);
+    slot = -1;
+  }
+  if (pos < 0 || pos >= a.num_positions) {
+    if (j == 0) set_status(a.c.status, NVB200_STATUS_BAD_POSITION);
+    pos = 0;
+  }
+  float c[8] = {}, sn[8] = {};
+  if (rotates) {
+    const float *cs = a.cos_sin + pos * a.cs_stride;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 cc = __ldg(reinterpret_cast<const float4 *>(cs + 8 * j) + i);
+      const float4 s4 = __ldg(reinterpret_cast<const float4 *>(cs + HALF + 8 * j) + i);
+      c[4 * i] = cc.x, c[4 * i + 1] = cc.y, c[4 * i + 2] = cc.z, c[4 * i + 3] = cc.w;
+      sn[4 * i] = s4.x, sn[4 * i + 1] = s4.y, sn[4 * i + 2] = s4.z, sn[4 * i + 3] = s4.w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int head = head0 + i;
     const bool is_q = head < a.hq, is_v = head >= a.hq + a.c.hkv;
     const int h = is_q ? head : (is_v ? head - a.hq - a.c.hkv : head - a.hq);
-    const __nv_bfloat16 *x = (is_q ? a.q + t * a.q_stride : (is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride)) +
-                             static_cast<int64_t>(h) * D;
-    uint4 xa = make_uint4(0, 0, 0, 0), xb = xa;
-    int64_t slot = -1;
-    if (live) {
-      xa = __ldg(reinterpret_cast<const uint4 *>(x + 8 * j));
-      xb = __ldg(reinterpret_cast<const uint4 *>(x + HALF + 8 * j));
-      if (!is_q) slot = __ldg(a.slots + t);
-    }
-    if (slot < -1 || slot >= a.c.num_slots) {
-      if (j == 0) set_status(a.c.status, NVB200_STATUS_BAD_SLOT);
-      slot = -1;
-    }
     float x1[8], x2[8];
-    unpack8(xa, x1);
-    unpack8(xb, x2);
+    unpack8(xa[i], x1);
+    unpack8(xb[i], x2);
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x1[i], x1[i], ss);
+    for (int e = 0; e < 8; ++e) ss = fmaf(x1[e], x1[e], ss);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x2[i], x2[i], ss);
+    for (int e = 0; e < 8; ++e) ss = fmaf(x2[e], x2[e], ss);
 #pragma unroll
     for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (live && !is_v) {
-      int64_t pos = __ldg(a.positions + t);
-      if (pos < 0 || pos >= a.num_positions) {
-        if (j == 0) set_status(a.c.status, NVB200_STATUS_BAD_POSITION);
-        pos = 0;
-      }
-      const float *cs = a.cos_sin + pos * a.cs_stride;
-      float c[8], sn[8];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float4 cc = __ldg(reinterpret_cast<const float4 *>(cs + 8 * j) + i);
-        const float4 s4 = __ldg(reinterpret_cast<const float4 *>(cs + HALF + 8 * j) + i);
-        c[4 * i] = cc.x, c[4 * i + 1] = cc.y, c[4 * i + 2] = cc.z, c[4 * i + 3] = cc.w;
-        sn[4 * i] = s4.x, sn[4 * i + 1] = s4.y, sn[4 * i + 2] = s4.z, sn[4 * i + 3] = s4.w;
-      }
+    if (!is_v) {
       uint32_t w1[4], w2[4];
       load_w8((is_q ? a.q_w : a.k_w) + 8 * j, w1);
       load_w8((is_q ? a.q_w : a.k_w) + HALF + 8 * j, w2);
       const float rstd = rsqrtf(ss / static_cast<float>(D) + a.eps);
       float y1[8], y2[8];
       norm_rope8(x1, x2, rstd, w1, w2, c, sn, y1, y2);
-      xa = pack8(y1), xb = pack8(y2);
+      xa[i] = pack8(y1), xb[i] = pack8(y2);
       __nv_bfloat16 *o = is_q ? a.q_out + (static_cast<int64_t>(t) * a.hq + h) * D
                               : (a.k_out ? a.k_out + (static_cast<int64_t>(t) * a.c.hkv + h) * D : nullptr);
       if (o) {
-        *reinterpret_cast<uint4 *>(o + 8 * j) = xa;
-        *reinterpret_cast<uint4 *>(o + HALF + 8 * j) = xb;
+        *reinterpret_cast<uint4 *>(o + 8 * j) = xa[i];
+        *reinterpret_cast<uint4 *>(o + HALF + 8 * j) = xb[i];
       }
     }
-    unpack8(xa, x1);
-    unpack8(xb, x2);
+    // A warp's groups may hold heads of different kinds; the shuffles below need all of its lanes.
+    if (__all_sync(0xffffffffu, is_q)) continue;
+    unpack8(xa[i], x1);
+    unpack8(xb[i], x2);
     uint32_t am = max(amax8(x1), amax8(x2));
 #pragma unroll
     for (int o = LPH / 2; o > 0; o >>= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
-    if (slot < 0) continue;
+    if (is_q || slot < 0 || head >= a.heads) continue;
     const RowScale rs = row_scale<FMT>(am);
     uint8_t *row = (is_v ? a.c.v : a.c.k) + (slot * a.c.hkv + h) * D;
     *reinterpret_cast<uint2 *>(row + 8 * j) = quantise8<FMT>(x1, rs);
@@ -277,16 +369,26 @@ __global__ void __launch_bounds__(kQuantThreads) qknr_quant_kernel(const __grid_
   }
 }
 
-template <int FMT> int launch_qknr_quant(const QknrQuantArgs &a, cudaStream_t s) {
-  const int lph = a.c.d / 16;
-  const int grid = grid_for(a.units, kQuantThreads / lph, 8);
+// R heads a group: 4 once that still fills the GPU.
+template <int D, int FMT> int launch_qknr_dim(QknrQuantArgs &a, int64_t tokens, cudaStream_t s) {
+  constexpr int64_t kGroups = kQuantThreads / (D / 16);
+  auto launch = [&](auto kernel, int r) {
+    a.by_parts.set(static_cast<uint32_t>((a.heads + r - 1) / r));
+    a.units = static_cast<uint32_t>(tokens * a.by_parts.d);
+    kernel<<<static_cast<unsigned>((a.units + kGroups - 1) / kGroups), kQuantThreads, 0, s>>>(a);
+    return launch_status();
+  };
+  if (tokens * a.heads > 4 * 4 * kGroups * sm_count()) return launch(qknr_quant_kernel<D, FMT, 4>, 4);
+  return launch(qknr_quant_kernel<D, FMT, 1>, 1);
+}
+
+template <int FMT> int launch_qknr_quant(QknrQuantArgs &a, int64_t tokens, cudaStream_t s) {
   switch (a.c.d) {
-    case 64: qknr_quant_kernel<64, FMT><<<grid, kQuantThreads, 0, s>>>(a); break;
-    case 128: qknr_quant_kernel<128, FMT><<<grid, kQuantThreads, 0, s>>>(a); break;
-    case 256: qknr_quant_kernel<256, FMT><<<grid, kQuantThreads, 0, s>>>(a); break;
-    default: return NVB200_ERR_UNSUPPORTED;
+    case 64: return launch_qknr_dim<64, FMT>(a, tokens, s);
+    case 128: return launch_qknr_dim<128, FMT>(a, tokens, s);
+    case 256: return launch_qknr_dim<256, FMT>(a, tokens, s);
   }
-  return launch_status();
+  return NVB200_ERR_UNSUPPORTED;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -303,6 +405,7 @@ struct LoadQuantArgs {
   int max_pages;
   int64_t num_blocks;
   int64_t total;
+  int run;        // tokens a warp takes, at most 32
   int zero_rest;  // rows outside every sequence: 1 = zeros, 0 = left as they are
   QuantCache c;
 };
@@ -344,50 +447,62 @@ NVB200_DEVICE int64_t slot_of_row(const LoadQuantArgs &a, int64_t t) {
   return blk * a.c.block_size + (pos - page * a.c.block_size);
 }
 
-// A warp takes 32 consecutive packed rows at a time: each lane looks up one row's slot (one search per token, not one
-// per head), then the warp copies the 32 tokens, the LPR lanes of a group one head's row at a time.
+// A warp takes a.run consecutive packed tokens at a time: lane i looks up the slot of token i (one search per token, not one
+// per head), then the warp copies their rows, the LPR lanes of a group one head's row at a time, U rows in flight.
 template <typename T, int FMT, int LPR>
 __global__ void __launch_bounds__(kQuantThreads) load_quant_kernel(const __grid_constant__ LoadQuantArgs a) {
-  constexpr int RPW = 32 / LPR;
-  const int lane = threadIdx.x & 31, j = lane % LPR, grp = lane / LPR;
-  const bool vec_on = 8 * j < a.c.d;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kQuantThreads / 32);
-  const int rows_in_token = a.c.hkv;
-  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (kQuantThreads / 32) + threadIdx.x / 32) * 8; t0 < a.total;
-       t0 += warps * 8) {
-    const int n = static_cast<int>(min(static_cast<int64_t>(8), a.total - t0));
-    int64_t mine = -1;
-    if (lane < n) {
-      mine = slot_of_row(a, t0 + lane);
-      if (mine == -2) set_status(a.c.status, NVB200_STATUS_BAD_SLOT);
-    }
-    for (int r = grp; r < n * rows_in_token + grp; r += RPW) {  // every group the same number of rounds
-      const int rr = min(r, n * rows_in_token - 1);
-      const int i = rr / rows_in_token, h = rr - i * rows_in_token;
-      const int64_t slot = __shfl_sync(0xffffffffu, mine, i);
-      if (r >= n * rows_in_token || !vec_on) continue;
-      const int64_t dst = ((t0 + i) * a.c.hkv + h) * a.c.d + 8 * j;
-      float k[8] = {}, v[8] = {};
-      if (slot >= 0) {
-        const int64_t src = (slot * a.c.hkv + h) * a.c.d + 8 * j;
-        const uint2 kw = __ldg(reinterpret_cast<const uint2 *>(a.c.k + src));
-        const uint2 vw = __ldg(reinterpret_cast<const uint2 *>(a.c.v + src));
-        const int64_t si = scale_index(a.c, slot, h);
-        const float ks = __ldg(a.c.k_scale + si), vs = __ldg(a.c.v_scale + si);
-        code_values8<FMT>(kw, k);
-        code_values8<FMT>(vw, v);
+  constexpr int RPW = 32 / LPR, U = 2;
+  const int lane = threadIdx.x & 31, j = lane % LPR, grp = lane / LPR, half = a.c.d / 2;
+  const bool on = 8 * j < half;
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (kQuantThreads / 32) + threadIdx.x / 32) * a.run;
+  if (t0 >= a.total) return;
+  const int n = static_cast<int>(min(static_cast<int64_t>(a.run), a.total - t0)), rows = n * a.c.hkv;
+  int64_t mine = -1;
+  if (lane < n) {
+    mine = slot_of_row(a, t0 + lane);
+    if (mine == -2) set_status(a.c.status, NVB200_STATUS_BAD_SLOT);
+  }
+  for (int r0 = 0; r0 < rows; r0 += RPW * U) {
+    uint2 kw[U][2], vw[U][2];
+    float ks[U], vs[U];
+    int64_t slot[U];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) k[e] *= ks, v[e] *= vs;
-      } else if (slot == -1 && !a.zero_rest) {
-        continue;
+    for (int x = 0; x < U; ++x) {
+      const int r = min(r0 + x * RPW + grp, rows - 1);
+      const int i = static_cast<int>(a.c.by_hkv.quotient(r)), h = r - i * a.c.hkv;
+      slot[x] = __shfl_sync(0xffffffffu, mine, i);
+      kw[x][0] = kw[x][1] = vw[x][0] = vw[x][1] = make_uint2(0, 0);
+      ks[x] = vs[x] = 0.f;
+      if (on && slot[x] >= 0) {
+        const int64_t src = (slot[x] * a.c.hkv + h) * a.c.d + 8 * j;
+        const int64_t si = scale_index(a.c, slot[x], h);
+        kw[x][0] = __ldg(reinterpret_cast<const uint2 *>(a.c.k + src));
+        kw[x][1] = __ldg(reinterpret_cast<const uint2 *>(a.c.k + src + half));
+        vw[x][0] = __ldg(reinterpret_cast<const uint2 *>(a.c.v + src));
+        vw[x][1] = __ldg(reinterpret_cast<const uint2 *>(a.c.v + src + half));
+        ks[x] = __ldg(a.c.k_scale + si), vs[x] = __ldg(a.c.v_scale + si);
       }
-      store8(static_cast<T *>(a.key) + dst, k);
-      store8(static_cast<T *>(a.value) + dst, v);
+    }
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      const int r = r0 + x * RPW + grp;
+      if (r >= rows || !on || (slot[x] == -1 && !a.zero_rest)) continue;
+      const int64_t dst = (t0 * a.c.hkv + r) * a.c.d + 8 * j;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float k[8], v[8];
+        code_values8<FMT>(kw[x][i], k);
+        code_values8<FMT>(vw[x][i], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[e] *= ks[x], v[e] *= vs[x];
+        store8(static_cast<T *>(a.key) + dst + i * half, k);
+        store8(static_cast<T *>(a.value) + dst + i * half, v);
+      }
     }
   }
 }
 
-// D not a multiple of 8 or above 256, or an address that is not 16-byte aligned: one warp per row of one tensor.
+// D not a multiple of 16 or above 512, or an address that is not 16-byte aligned: one warp per row of one tensor.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kQuantThreads) load_quant_any_kernel(const __grid_constant__ LoadQuantArgs a) {
   const int lane = threadIdx.x & 31;
@@ -409,22 +524,24 @@ __global__ void __launch_bounds__(kQuantThreads) load_quant_any_kernel(const __g
   }
 }
 
-template <typename T, int FMT> int launch_load_quant(const LoadQuantArgs &a, bool vec, cudaStream_t s) {
+template <typename T, int FMT> int launch_load_quant(LoadQuantArgs &a, bool vec, cudaStream_t s) {
   if (!vec) {
     load_quant_any_kernel<T, FMT>
         <<<grid_for(2 * a.total * a.c.hkv, kQuantThreads / 32, 8), kQuantThreads, 0, s>>>(a);
     return launch_status();
   }
-  const int lanes = a.c.d / 8;
-  const int lpr = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : 32);
-  const int grid = grid_for(a.total, 8 * (kQuantThreads / 32), 8);
-  if (lpr == 8) load_quant_kernel<T, FMT, 8><<<grid, kQuantThreads, 0, s>>>(a);
-  else if (lpr == 16) load_quant_kernel<T, FMT, 16><<<grid, kQuantThreads, 0, s>>>(a);
-  else load_quant_kernel<T, FMT, 32><<<grid, kQuantThreads, 0, s>>>(a);
-  return launch_status();
+  // Tokens a warp: as many as leave every SM its 64 warps, 8 at most (more gain nothing).
+  const int64_t warps = static_cast<int64_t>(sm_count()) * 64;
+  a.run = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, a.total / warps)));
+  const int64_t per_cta = static_cast<int64_t>(a.run) * (kQuantThreads / 32);
+  const unsigned grid = static_cast<unsigned>((a.total + per_cta - 1) / per_cta);
+  return with_lanes(a.c.d, [&](auto lanes) {
+    load_quant_kernel<T, FMT, lanes()><<<grid, kQuantThreads, 0, s>>>(a);
+    return launch_status();
+  });
 }
 
-template <typename T> int launch_load_fmt(const LoadQuantArgs &a, int fmt, bool vec, cudaStream_t s) {
+template <typename T> int launch_load_fmt(LoadQuantArgs &a, int fmt, bool vec, cudaStream_t s) {
   return fmt == kCacheE4M3 ? launch_load_quant<T, kCacheE4M3>(a, vec, s) : launch_load_quant<T, kCacheI8>(a, vec, s);
 }
 
@@ -444,6 +561,7 @@ int prepare_cache(const nvb200_quant_cache *q, int32_t *status, QuantCache &c, i
   c.k_scale = q->k_scale, c.v_scale = q->v_scale;
   c.num_slots = q->num_blocks * q->block_size;
   c.block_size = q->block_size, c.hkv = q->num_kv_heads, c.d = q->head_dim;
+  c.by_block.set(static_cast<uint32_t>(q->block_size)), c.by_hkv.set(static_cast<uint32_t>(q->num_kv_heads));
   c.status = status;
   return NVB200_OK;
 }
@@ -475,7 +593,7 @@ extern "C" int nvb200_store_kvcache_quant(const void *key, int64_t key_token_str
   a.key_stride = key_token_stride, a.value_stride = value_token_stride;
   a.slots = slot_mapping, a.slot64 = slot_bytes == 8;
   a.rows = static_cast<uint32_t>(num_tokens * a.c.hkv);
-  const bool vec = a.c.d % 8 == 0 && a.c.d <= 256 && aligned16(key) && aligned16(value) &&
+  const bool vec = fits_lanes(a.c.d) && aligned16(key) && aligned16(value) &&
                    multiple16(key_token_stride * es) && multiple16(value_token_stride * es) && aligned16(a.c.k) &&
                    aligned16(a.c.v);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -516,10 +634,11 @@ extern "C" int nvb200_qk_norm_rope_kv_quant(const nvb200_qk_norm_rope_kv_args *q
   a.q_w = static_cast<const B *>(q->q_weight), a.k_w = static_cast<const B *>(q->k_weight);
   a.cos_sin = q->cos_sin, a.cs_stride = q->cos_sin_stride, a.num_positions = q->num_positions;
   a.q_out = static_cast<B *>(q->q_out), a.k_out = static_cast<B *>(q->k_out);
-  a.units = static_cast<uint32_t>(q->num_tokens * heads), a.hq = q->num_q_heads, a.heads = static_cast<int>(heads);
+  a.hq = q->num_q_heads, a.heads = static_cast<int>(heads);
   a.eps = q->eps;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return fmt == kCacheE4M3 ? launch_qknr_quant<kCacheE4M3>(a, s) : launch_qknr_quant<kCacheI8>(a, s);
+  return fmt == kCacheE4M3 ? launch_qknr_quant<kCacheE4M3>(a, q->num_tokens, s)
+                           : launch_qknr_quant<kCacheI8>(a, q->num_tokens, s);
 }
 
 extern "C" int nvb200_load_kvcache_quant(void *key, void *value, const nvb200_quant_cache *cache,
@@ -540,7 +659,7 @@ extern "C" int nvb200_load_kvcache_quant(void *key, void *value, const nvb200_qu
   a.key = key, a.value = value, a.table = block_table, a.table_stride = block_table_stride, a.cu = cu_seqlens;
   a.batch = batch, a.max_pages = max_blocks_per_seq, a.num_blocks = cache->num_blocks, a.total = total_tokens;
   a.zero_rest = zero_rest;
-  const bool vec = a.c.d % 8 == 0 && a.c.d <= 256 && aligned16(key) && aligned16(value) && aligned16(a.c.k) &&
+  const bool vec = fits_lanes(a.c.d) && aligned16(key) && aligned16(value) && aligned16(a.c.k) &&
                    aligned16(a.c.v);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == NVB200_BF16) return launch_load_fmt<__nv_bfloat16>(a, fmt, vec, s);

@@ -27,6 +27,7 @@ struct RowScale {
   float scale;  // what is stored (NaN for a row that is not finite)
   float mul;    // e4m3: 2^-E. int8: 127 (times 2^-8 for rows above 2^100, so that 127 x stays finite)
   float den;    // int8: d, times the same factor
+  float quot;   // int8: 127 / d rounded (at most 2^126: finite)
   bool finite;
 };
 
@@ -40,16 +41,22 @@ template <int FMT> NVB200_DEVICE RowScale row_scale(uint32_t amax_bits) {
     E = E < -126 ? -126 : E;
     r.scale = __uint_as_float(static_cast<uint32_t>(E + 127) << 23);
     r.mul = __uint_as_float(static_cast<uint32_t>(127 - E) << 23);
-    r.den = 1.f;
+    r.den = r.quot = 1.f;
   } else {
     const float d = fmaxf(__uint_as_float(amax_bits), 127.f * 1.17549435e-38f);
     r.scale = __fdiv_rn(d, 127.f);
     const float h = d > 1.2676506e30f ? 0.00390625f : 1.f;  // 2^100, 2^-8
     r.mul = 127.f * h;
     r.den = d * h;
+    r.quot = __fdiv_rn(127.f, d);
   }
   if (!r.finite) r.scale = __uint_as_float(0x7FC00000u);
   return r;
+}
+
+// int8: the code by the correctly rounded quotient, in the low byte.
+NVB200_DEVICE uint32_t exact_code(float x, const RowScale &r) {
+  return static_cast<uint32_t>(__float2int_rn(__fdiv_rn(__fmul_rn(x, r.mul), r.den)));
 }
 
 // Eight elements to eight codes, element 0 in the lowest byte.
@@ -60,12 +67,24 @@ template <int FMT> NVB200_DEVICE uint2 quantise8(const float (&x)[8], const RowS
     out.x = pack_e4m3x2(x[0] * r.mul, x[1] * r.mul) | pack_e4m3x2(x[2] * r.mul, x[3] * r.mul) << 16;
     out.y = pack_e4m3x2(x[4] * r.mul, x[5] * r.mul) | pack_e4m3x2(x[6] * r.mul, x[7] * r.mul) << 16;
   } else {
+    // x times the row's 127 / d, rounded at the unit by adding 1.5 * 2^23 (the code is then the sum's low byte). Two
+    // roundings of 2^-24 and the quotient's own move a value of at most 127 by less than 3 * 127 * 2^-24 < kNear, so
+    // where no product lies that near to the middle between two codes, they are the quotient's codes; else it is taken.
+    constexpr float kMagic = 12582912.f, kNear = 127.f * 2.384185791015625e-7f;  // 2^-22
     uint32_t c[8];
+    float off = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      c[i] = static_cast<uint32_t>(__float2int_rn(__fdiv_rn(__fmul_rn(x[i], r.mul), r.den))) & 0xFFu;
-    out.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-    out.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
+    for (int i = 0; i < 8; ++i) {
+      const float p = __fmul_rn(x[i], r.quot), m = __fadd_rn(p, kMagic);
+      off = fmaxf(off, fabsf(__fsub_rn(p, __fsub_rn(m, kMagic))));
+      c[i] = __float_as_uint(m);
+    }
+    if (off > 0.5f - kNear) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = exact_code(x[i], r);
+    }
+    out.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    out.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
   }
   return out;
 }
@@ -76,7 +95,7 @@ template <int FMT> NVB200_DEVICE uint8_t quantise1(float x, const RowScale &r) {
   if constexpr (FMT == kCacheE4M3)
     return static_cast<uint8_t>(pack_e4m3x2(x * r.mul, 0.f) & 0xFFu);
   else
-    return static_cast<uint8_t>(static_cast<uint32_t>(__float2int_rn(__fdiv_rn(__fmul_rn(x, r.mul), r.den))) & 0xFFu);
+    return static_cast<uint8_t>(exact_code(x, r) & 0xFFu);
 }
 
 // Two e4m3 codes (low byte first) as two fp16 values: exact, every e4m3 value is an fp16 value.
