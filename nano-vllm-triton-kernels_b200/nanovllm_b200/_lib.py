@@ -6,6 +6,7 @@ CUDA device (int32, zeroed at creation) receives the kernels' NVB200_STATUS_* bi
 """
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -70,7 +71,22 @@ class PagedDecodeArgs(ctypes.Structure):
     ]
 
 
-class QuantCache(ctypes.Structure):
+_CODES = {_vp: "P", _i64: "q", _i32: "i", _f32: "f"}
+
+
+class _Packed(ctypes.Structure):
+    """A C struct that calls also take as the bytes of pack(...), its fields in order (a null pointer is 0): that costs a
+    third of what filling the structure does, which counts where a call's host time exceeds its kernel's."""
+
+    def __init_subclass__(cls):
+        cls.pack = struct.Struct("@" + "".join(_CODES[t] for _, t in cls._fields_)).pack
+
+    @classmethod
+    def from_param(cls, x):
+        return ctypes.byref(x) if isinstance(x, cls) else x
+
+
+class QuantCache(_Packed):
     """nvb200_quant_cache (field order and types as in nvb200.h)."""
     _fields_ = [
         ("k_cache", _vp), ("v_cache", _vp), ("k_scale", _vp), ("v_scale", _vp), ("num_blocks", _i64),
@@ -78,7 +94,7 @@ class QuantCache(ctypes.Structure):
     ]
 
 
-class CacheAttentionArgs(ctypes.Structure):
+class CacheAttentionArgs(_Packed):
     """nvb200_cache_attention_args (field order and types as in nvb200.h)."""
     _fields_ = [
         ("out", _vp), ("q", _vp), ("q_batch_stride", _i64), ("q_token_stride", _i64), ("q_head_stride", _i64),
@@ -155,17 +171,17 @@ def _declare(lib):
     lib.nvb200_paged_decode_attention_streamk.restype = ctypes.c_int
     lib.nvb200_paged_decode_attention_noalloc.argtypes = [ctypes.POINTER(PagedDecodeArgs), _vp]
     lib.nvb200_paged_decode_attention_noalloc.restype = ctypes.c_int
-    lib.nvb200_store_kvcache_quant.argtypes = [_vp, _i64, _vp, _i64, _vp, ctypes.c_int, _i64, ctypes.c_int,
-                                               ctypes.POINTER(QuantCache), _vp, _vp]
+    lib.nvb200_store_kvcache_quant.argtypes = [_vp, _i64, _vp, _i64, _vp, ctypes.c_int, _i64, ctypes.c_int, QuantCache,
+                                               _vp, _vp]
     lib.nvb200_store_kvcache_quant.restype = ctypes.c_int
-    lib.nvb200_qk_norm_rope_kv_quant.argtypes = [ctypes.POINTER(QkNormRopeKvArgs), ctypes.POINTER(QuantCache), _vp]
+    lib.nvb200_qk_norm_rope_kv_quant.argtypes = [ctypes.POINTER(QkNormRopeKvArgs), QuantCache, _vp]
     lib.nvb200_qk_norm_rope_kv_quant.restype = ctypes.c_int
-    lib.nvb200_load_kvcache_quant.argtypes = [_vp, _vp, ctypes.POINTER(QuantCache), _vp, _i64, _i32, _vp, _i32, _i64,
-                                              ctypes.c_int, ctypes.c_int, _vp, _vp]
+    lib.nvb200_load_kvcache_quant.argtypes = [_vp, _vp, QuantCache, _vp, _i64, _i32, _vp, _i32, _i64, ctypes.c_int,
+                                              ctypes.c_int, _vp, _vp]
     lib.nvb200_load_kvcache_quant.restype = ctypes.c_int
-    lib.nvb200_cache_attention_workspace_size.argtypes = [ctypes.POINTER(CacheAttentionArgs)]
+    lib.nvb200_cache_attention_workspace_size.argtypes = [CacheAttentionArgs]
     lib.nvb200_cache_attention_workspace_size.restype = _i64
-    lib.nvb200_cache_attention.argtypes = [ctypes.POINTER(CacheAttentionArgs), _vp, _i64, _vp]
+    lib.nvb200_cache_attention.argtypes = [CacheAttentionArgs, _vp, _i64, _vp]
     lib.nvb200_cache_attention.restype = ctypes.c_int
 
 
@@ -194,7 +210,7 @@ def check(rc: int, what: str) -> None:
 
 def stream_of(t: torch.Tensor) -> int:
     """The current torch stream of t's device (kernels launch there, as Triton's do)."""
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 class _SameDevice:

@@ -27,9 +27,10 @@ def _require(cond: bool, msg: str = "") -> None:
 
 def _run(what, q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, tree_mask, draft_lens, softmax_scale,
          causal, num_splits):
-    _require(q.dim() == 4 and q.stride(3) == 1 and q.is_cuda, "q must be a CUDA tensor [B, n, Hq, D], unit last stride")
+    sq = q.stride()
+    _require(len(sq) == 4 and sq[3] == 1 and q.is_cuda, "q must be a CUDA tensor [B, n, Hq, D], unit last stride")
     B, n, hq, d = q.shape
-    dev = q.device
+    dev, idx = q.device, q.get_device()
     if k_scale is None and v_scale is None:
         _require(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and v_cache.stride() == k_cache.stride()
                  and k_cache.stride(3) == 1, "the caches must be [blocks, block_size, Hkv, D] of equal strides, unit last")
@@ -38,7 +39,7 @@ def _run(what, q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table
         if k_cache.dtype != q.dtype:
             raise NotImplementedError(f"{what}: a 16-bit cache must have q's dtype")
         nb, bs, hkv, dk = k_cache.shape
-        code, scales = _QUERY.get(q.dtype), (None, None)
+        code, scales = _QUERY.get(q.dtype), (0, 0)
     else:
         _require(k_scale is not None and v_scale is not None, "k_scale and v_scale come together")
         nb, bs, hkv, dk = check_quant_cache(k_cache, v_cache, k_scale, v_scale)
@@ -53,19 +54,19 @@ def _run(what, q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table
         raise NotImplementedError(f"{what}: at most {MAX_NEW_TOKENS} new tokens per sequence")
     _require(0 <= num_splits <= 8, "num_splits must be 0 (automatic) to 8")
     _require(cache_seqlens.shape == (B,) and cache_seqlens.dtype == torch.int32, "cache_seqlens must be int32 [B]")
-    _require(k_cache.device == dev and v_cache.device == dev and cache_seqlens.device == dev,
+    _require(k_cache.get_device() == v_cache.get_device() == cache_seqlens.get_device() == idx,
              "q, the caches and cache_seqlens must be on one device")
     seqlens = cache_seqlens if cache_seqlens.is_contiguous() else cache_seqlens.contiguous()
     if block_table is not None:
         _require(block_table.dim() == 2 and block_table.shape[0] == B and block_table.shape[1] > 0
-                 and block_table.dtype == torch.int32 and block_table.device == dev
+                 and block_table.dtype == torch.int32 and block_table.get_device() == idx
                  and (block_table.stride(1) == 1 or block_table.shape[1] == 1),
                  "block_table must be int32 [B, max_blocks] on q's device")
         table, table_stride, pages = block_table.data_ptr(), block_table.stride(0), block_table.shape[1]
     else:
         _require(nb >= B, "without a block_table the cache must have a block for each sequence")
-        table, table_stride, pages = None, 0, 1
-    mask, mask_b, mask_r = None, 0, 0
+        table, table_stride, pages = 0, 0, 1
+    mask, mask_b, mask_r, drafts = 0, 0, 0, 0
     if tree_mask is not None:
         _require(tree_mask.dtype == torch.bool and tree_mask.device == dev, "tree_mask must be bool on q's device")
         if tree_mask.dim() == 2:
@@ -81,13 +82,14 @@ def _run(what, q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table
         _require(draft_lens.shape == (B,) and draft_lens.dtype == torch.int32 and draft_lens.device == dev,
                  "draft_lens must be int32 [B] on q's device")
         draft_lens = draft_lens if draft_lens.is_contiguous() else draft_lens.contiguous()
-    out = torch.empty(B, n, hq, d, dtype=q.dtype, device=dev)
+        drafts = draft_lens.data_ptr()
+    out = torch.empty((B, n, hq, d), dtype=q.dtype, device=dev)
     if B == 0 or n == 0:
         return out
-    sq, sk = q.stride(), k_cache.stride()
-    a = _lib.CacheAttentionArgs(
+    sk = k_cache.stride()
+    a = _lib.CacheAttentionArgs.pack(
         out.data_ptr(), q.data_ptr(), sq[0], sq[1], sq[2], k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2],
-        scales[0], scales[1], nb, table, table_stride, seqlens.data_ptr(), _lib.ptr(draft_lens), mask, mask_b, mask_r,
+        scales[0], scales[1], nb, table, table_stride, seqlens.data_ptr(), drafts, mask, mask_b, mask_r,
         B, n, hq, hkv, d, bs, pages, int(bool(causal)), int(num_splits), _QUERY[q.dtype], code,
         d ** -0.5 if softmax_scale is None else float(softmax_scale), _lib.status_word(dev).data_ptr())
     L = _lib.lib()

@@ -44,21 +44,22 @@ def empty_quant_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_
 def check_quant_cache(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int]:
     """Checks the four tensors of an 8-bit cache; (blocks, block_size, Hkv, D)."""
     shape = k_cache.shape
-    _require(len(shape) == 4 and k_cache.dtype in _lib.QUANT_CODE and v_cache.dtype == k_cache.dtype
-             and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous(),
+    dtype = k_cache.dtype
+    _require(len(shape) == 4 and dtype in _lib.QUANT_CODE and v_cache.dtype == dtype and v_cache.shape == shape
+             and k_cache.is_contiguous() and v_cache.is_contiguous(),
              "k_cache, v_cache must be contiguous [blocks, block_size, Hkv, D] float8_e4m3fn or int8")
     blocks, bs, hkv, d = shape
-    _require(k_scale.dtype == v_scale.dtype == torch.float32 and k_scale.shape == v_scale.shape == (blocks, hkv, bs)
-             and k_scale.is_contiguous() and v_scale.is_contiguous(),
+    scale_shape = k_scale.shape
+    _require(k_scale.dtype is v_scale.dtype is torch.float32 and scale_shape == (blocks, hkv, bs)
+             and v_scale.shape == scale_shape and k_scale.is_contiguous() and v_scale.is_contiguous(),
              "k_scale, v_scale must be contiguous fp32 [blocks, Hkv, block_size]")
-    dev = k_cache.device
-    _require(v_cache.device == dev and k_scale.device == dev and v_scale.device == dev,
+    _require(k_cache.get_device() == v_cache.get_device() == k_scale.get_device() == v_scale.get_device(),
              "the cache's tensors must be on one device")
     return blocks, bs, hkv, d
 
 
 def _cache_arg(k_cache, v_cache, k_scale, v_scale, shape):
-    return _lib.QuantCache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *shape,
+    return _lib.QuantCache.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *shape,
                            _lib.QUANT_CODE[k_cache.dtype])
 
 
@@ -70,22 +71,23 @@ def store_kvcache_quant(key: torch.Tensor, value: torch.Tensor, k_cache: torch.T
     _require(key.dim() == 3 and value.shape == key.shape and value.dtype == key.dtype, "key, value must be [N, Hkv, D]")
     _require(key.dtype in _lib.DTYPE_CODE, "dtype must be bf16, fp16 or fp32")
     n, hkv, d = key.shape
-    for x in (key, value):
-        _require(x.stride(2) == 1 and x.stride(1) == d, "each head must be contiguous: stride(2) == 1, stride(1) == D")
+    key_strides, value_strides = key.stride(), value.stride()
+    _require(key_strides[1:] == value_strides[1:] == (d, 1),
+             "each head must be contiguous: stride(2) == 1, stride(1) == D")
     shape = check_quant_cache(k_cache, v_cache, k_scale, v_scale)
     _require(shape[2:] == (hkv, d), "the cache must hold rows of the key's Hkv and D")
     _require(slot_mapping.shape == (n,) and slot_mapping.dtype in _SLOT_BYTES, "slot_mapping must be int32 or int64 [N]")
     _require(key.is_cuda, "key must be a CUDA tensor")
-    dev = key.device
-    _require(value.device == dev and k_cache.device == dev and slot_mapping.device == dev,
+    _require(key.get_device() == value.get_device() == k_cache.get_device() == slot_mapping.get_device(),
              "key, value, the cache and slot_mapping must be on one device")
+    dev = key.device
     if n == 0:
         return
     slots = slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
     cache = _cache_arg(k_cache, v_cache, k_scale, v_scale, shape)
     with _lib.device_of(dev):
         _lib.check(_lib.lib().nvb200_store_kvcache_quant(
-            key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), slots.data_ptr(),
+            key.data_ptr(), key_strides[0], value.data_ptr(), value_strides[0], slots.data_ptr(),
             _SLOT_BYTES[slots.dtype], n, _lib.DTYPE_CODE[key.dtype], cache, _lib.status_word(dev).data_ptr(),
             _lib.stream_of(key)), "store_kvcache_quant")
 
@@ -103,8 +105,8 @@ def qk_norm_rope_kv_quant(
     _require(q.dtype == k.dtype == v.dtype == torch.bfloat16 and k.shape == v.shape == (T, Hkv, D),
              "q, k, v must be bf16 with k.shape == v.shape == (T, Hkv, D)")
     _require(Hkv > 0 and Hq % Hkv == 0 and D % 2 == 0, "Hq must be a multiple of Hkv and D even")
-    for x in (q, k, v):
-        _require(x.stride(2) == 1 and x.stride(1) == D, "each head must be contiguous: stride(2) == 1, stride(1) == D")
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    _require(sq[1:] == sk[1:] == sv[1:] == (D, 1), "each head must be contiguous: stride(2) == 1, stride(1) == D")
     _require(positions.shape == (T,) and positions.dtype == torch.int64 and positions.is_contiguous(),
              "positions must be contiguous int64 [T]")
     _require(cos_sin_cache.dtype == torch.float32 and cos_sin_cache.shape[-1] == D and cos_sin_cache.stride(-1) == 1
@@ -116,17 +118,17 @@ def qk_norm_rope_kv_quant(
     _require(shape[2:] == (Hkv, D), "the cache must hold rows of k's Hkv and D")
     _require(slot_mapping.shape == (T,) and slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous(),
              "slot_mapping must be contiguous int32 [T]")
-    dev = q.device
+    dev, idx = q.device, q.get_device()
     _require(q.is_cuda, "q must be a CUDA tensor")
     for x in (k, v, positions, q_weight, k_weight, cos_sin_cache, k_cache, slot_mapping):
-        _require(x.device == dev, "all tensors must be on one device")
+        _require(x.get_device() == idx, "all tensors must be on one device")
     q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
     k_out = torch.empty(T, Hkv, D, dtype=q.dtype, device=dev) if write_k else None
     if T == 0:
         return q_out, k_out
     a = _lib.QkNormRopeKvArgs(
-        q_out.data_ptr(), _lib.ptr(k_out), q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0),
-        v.stride(0), positions.data_ptr(), slot_mapping.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+        q_out.data_ptr(), _lib.ptr(k_out), q.data_ptr(), k.data_ptr(), v.data_ptr(), sq[0], sk[0], sv[0],
+        positions.data_ptr(), slot_mapping.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
         cos_sin_cache.data_ptr(), cos_sin_cache.stride(0), cos_sin_cache.shape[0], None, None, 0, T, Hq, Hkv, D, eps,
         _lib.status_word(dev).data_ptr())
     cache = _cache_arg(k_cache, v_cache, k_scale, v_scale, shape)
