@@ -538,3 +538,109 @@ def test_offsets_past_32_bits(cuda, cdt):
     kv = [s.float() * (0.5 if cdt == E4M3 else 1.0) for s in small]
     at = torch.arange(len(used)).view(2, pages).int()
     _check(got, q, kv, at, [L, L - 7], m[None].expand(2, n, n), [n, n], d ** -0.5, cdt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qdt,cdt", [(B16, B16), (H16, H16), (B16, E4M3), (H16, I8)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,hq,hkv,lens,drafts", [
+    (1, 8, 2, [4500, 1, 0, 700, 2100], None), (3, 8, 2, [5000, 2, 0, 700, 2100], [3, 2, 0, 1, 3]),
+    (6, 8, 1, [5000, 64, 47, 0, 129], None), (12, 8, 2, [4300, 11, 900], [12, 12, 7]),
+    (34, 8, 2, [3000, 34, 0, 5], [34, 30, 0, 34]), (100, 4, 2, [4200, 101, 100], None)])
+def test_shares_of_long_tables(cuda, qdt, cdt, d, n, hq, hkv, lens, drafts):
+    """Block tables long enough for the keys of all sequences to be dealt out evenly, in each size of row block: 1 to 8, 16,
+    several blocks of 16, 64 (16-bit caches) and 128."""
+    import nanovllm_b200
+    q, kv, cache, table, m, dr = _problem(len(lens), n, lens, hq, hkv, d, 64, qdt, cdt, cuda, seed=n, drafts=drafts)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    nanovllm_b200.status(cuda, clear=True)
+    run = lambda splits=0: nanovllm_b200.tree_attention(  # noqa: E731
+        q.to(cuda), cache[0], cache[1], i32(lens), m.to(cuda), table.to(cuda), None if drafts is None else i32(drafts),
+        k_scale=cache[2], v_scale=cache[3], num_splits=splits)
+    got = run()
+    _check(got, q, kv, table, lens, m, dr, d ** -0.5, cdt)
+    assert torch.equal(run(), got)
+    _check(run(3), q, kv, table, lens, m, dr, d ** -0.5, cdt)
+    assert nanovllm_b200.status(cuda) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cdt", [B16, E4M3])
+@pytest.mark.parametrize("n,hq", [(1, 4), (4, 4), (30, 4), (80, 4)])
+def test_many_short_sequences_in_wide_tables(cuda, cdt, n, hq):
+    """Shares that hold many sequences of a tile or less, pages of several sizes; the table's unused entries are never read."""
+    import nanovllm_b200
+    g = torch.Generator().manual_seed(n)
+    lens = [n + int(x) for x in torch.randint(0, 90, (70,), generator=g)]
+    q, kv, cache, table, m, drafts = _problem(70, n, lens, hq, 2, 64, 32, B16, cdt, cuda, seed=n)
+    wide = torch.full((70, 150), -7, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    nanovllm_b200.status(cuda, clear=True)
+    got = nanovllm_b200.tree_attention(q.to(cuda), cache[0], cache[1], torch.tensor(lens, dtype=torch.int32, device=cuda),
+                                       m.to(cuda), wide.to(cuda), k_scale=cache[2], v_scale=cache[3])
+    _check(got, q, kv, table, lens, m, drafts, 64 ** -0.5, cdt)
+    assert nanovllm_b200.status(cuda) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cdt", [B16, I8])
+@pytest.mark.parametrize("n", [2, 40, 80])
+def test_workspaces(cuda, cdt, n):
+    """The C call: a workspace that is too small or misaligned is refused, none at all gives the result by another form, and
+    nothing outside the stated bytes is written."""
+    import nanovllm_b200
+    from nanovllm_b200 import _lib
+    lens, d, scale = [4500, n], 128, 0.1
+    q, kv, cache, table, _, drafts = _problem(2, n, lens, 4, 2, d, 64, B16, cdt, cuda, mask=None)
+    qd, td, ld = q.to(cuda), table.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+    out = torch.zeros_like(qd)
+    s, k = qd.stride(), cache[0].stride()
+    a = _lib.CacheAttentionArgs.pack(
+        out.data_ptr(), qd.data_ptr(), s[0], s[1], s[2], cache[0].data_ptr(), cache[1].data_ptr(), k[0], k[1], k[2],
+        cache[2].data_ptr() if cdt == I8 else 0, cache[3].data_ptr() if cdt == I8 else 0, cache[0].shape[0], td.data_ptr(),
+        td.stride(0), ld.data_ptr(), 0, 0, 0, 0, 2, n, 4, 2, d, 64, td.shape[1], 1, 0, _lib.BF16,
+        _lib.I8 if cdt == I8 else _lib.BF16, scale, _lib.status_word(cuda).data_ptr())
+    L = _lib.lib()
+    need = L.nvb200_cache_attention_workspace_size(a)
+    assert need > 0
+    ws = torch.full((need + 64,), 77, dtype=torch.uint8, device=cuda)
+    stream = _lib.stream_of(qd)
+    assert L.nvb200_cache_attention(a, ws.data_ptr(), need - 1, stream) == _lib.ERR_ARG
+    assert L.nvb200_cache_attention(a, ws.data_ptr() + 8, need, stream) == _lib.ERR_ARG
+    assert L.nvb200_cache_attention(a, ws.data_ptr(), -1, stream) == _lib.ERR_ARG
+    assert not bool(out.any()) and bool((ws == 77).all())
+    for pointer, size in ((ws.data_ptr(), need), (None, 0)):
+        out.zero_()
+        assert L.nvb200_cache_attention(a, pointer, size, stream) == _lib.OK
+        _check(out, q, kv, table, lens, None, drafts, scale, cdt)
+    assert bool((ws[need:] == 77).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 40, 80])
+def test_two_calls_at_once(cuda, n):
+    """Calls in flight on two streams, eager and captured, keep to their own workspaces."""
+    import nanovllm_b200
+    lens = [4500, 300, 2000]
+    runs = []
+    for seed, cdt in ((1, B16), (2, E4M3)):
+        q, kv, cache, table, m, _ = _problem(3, n, lens, 8, 2, 128, 64, B16, cdt, cuda, seed=seed)
+        q, table, m, ld = q.to(cuda), table.to(cuda), m.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+        runs.append(lambda q=q, cache=cache, table=table, m=m, ld=ld: nanovllm_b200.tree_attention(
+            q, cache[0], cache[1], ld, m, table, k_scale=cache[2], v_scale=cache[3]))
+    want = [f().clone() for f in runs]
+    graphs, got = [], []
+    for f in runs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(f())
+    torch.cuda.synchronize()
+    streams, eager = [torch.cuda.Stream() for _ in runs], [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i].replay()
+                eager[i].append(runs[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(got[i], want[i]) and all(torch.equal(x, want[i]) for x in eager[i])

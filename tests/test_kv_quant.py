@@ -419,3 +419,48 @@ def test_offsets_past_32_bits(cuda):
     want = c.float() * s[..., None]
     assert torch.equal(k[[255, 256, 0]].cpu(), want) and not bool(k[1:255].any())
     assert int((cache[2] != 0).sum()) == 3 * hkv
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,hkv,d,bs", [(50, 3, 512, 16), (41, 2, 320, 5), (60, 1, 48, 16), (3, 7, 16, 256), (12, 2, 528, 8)])
+def test_other_row_widths_and_back(cuda, fmt, dtype, T, hkv, d, bs):
+    """Head dims that fill a group of lanes in part, and the first one past the widest group; written and read back."""
+    import nanovllm_b200
+    pages = -(-T // bs)
+    cache = _cache(pages + 1, bs, hkv, d, fmt, cuda)
+    table = torch.randperm(pages + 1, generator=torch.Generator().manual_seed(9))[:pages].int()
+    j = torch.arange(T)
+    slots = table[j // bs].long() * bs + j % bs
+    k, v = _rows(T, hkv, d, dtype, 4), _rows(T, hkv, d, dtype, 5)
+    want = _expect_store(cache, k, v, slots, bs)
+    nanovllm_b200.store_kvcache_quant(k.to(cuda), v.to(cuda), *cache, slots.to(cuda))
+    _same(cache, want)
+    got = nanovllm_b200.load_kvcache_quant(*cache, table.view(1, -1).to(cuda), torch.tensor([0, T], dtype=torch.int32,
+                                                                                            device=cuda), T, dtype=dtype)
+    for x, codes, scale in ((got[0], cache[0], cache[2]), (got[1], cache[1], cache[3])):
+        values = (codes.float() * scale.transpose(1, 2)[..., None]).to(dtype)
+        assert torch.equal(x, values[table.long().to(cuda)].flatten(0, 1)[:T])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("T,hq,hkv,d", [(1001, 32, 8, 128), (9001, 3, 1, 128), (4500, 16, 2, 64), (3000, 5, 1, 256)])
+def test_fused_many_tokens_equals_its_two_steps(cuda, fmt, T, hq, hkv, d):
+    """Enough tokens for a lane group to take several heads of one, head counts that they do not divide included."""
+    import nanovllm_b200
+    x = _fused_inputs(T, hq, hkv, d, cuda)
+    blocks = T // 144 + 1
+    a, b = _cache(blocks, 144, hkv, d, fmt, cuda), _cache(blocks, 144, hkv, d, fmt, cuda)
+    slots = torch.randperm(blocks * 144, generator=torch.Generator().manual_seed(7))[:T].int()
+    slots[::7] = -1
+    slots = slots.to(cuda)
+    none = x[0].new_empty(0)
+    q1, k1 = nanovllm_b200.qk_norm_rope_kv(*x, none, none, None, True)
+    nanovllm_b200.store_kvcache_quant(k1, x[2], *a, slots)
+    nanovllm_b200.status(cuda, clear=True)
+    q2, k2 = nanovllm_b200.qk_norm_rope_kv_quant(*x, *b, slots, True)
+    assert torch.equal(q1, q2) and torch.equal(k1, k2)
+    _same(a, [_bits(t).cpu() for t in b])
+    assert nanovllm_b200.status(cuda) == 0
