@@ -129,7 +129,8 @@ template <int CT, int D, int NT> NVB200_DEVICE bool clean_v_tile(uint32_t kt, in
 // Folds one tile. kt: the stage's base address. see[n][e]: which of the tile's keys that row sees, where `edge`; elsewhere
 // every row sees every key.
 template <int CT, int D, int NT>
-NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<D, NT> &q, int lane, bool edge, const uint32_t (&see)[NT][2]) {
+NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<D, NT> &q, int lane, bool edge,
+                             const uint32_t (&see)[NT][2]) {
   using G = Geometry<CT, D, NT>;
   using C = CacheType<CT>;
   constexpr int KB = G::kTile / 16;  // 16-key blocks
@@ -664,8 +665,8 @@ template <typename Kernel> int allow_smem(Kernel kernel, int bytes, std::atomic<
   return NVB200_OK;
 }
 
-// Largest power of two of CTAs per cluster that the longest possible sequence feeds with a tile for every other warp, while the clusters
-// fit on the GPU at once.
+// Largest power of two of CTAs per cluster that the longest possible sequence feeds with a tile for every other warp, while
+// the clusters fit on the GPU at once (one sequence of 611 keys: 4 CTAs 8.0 us, 8 CTAs 7.0 us).
 int cluster_splits(const CacheAttnParams &p, int64_t units, int tile, int ctas_per_sm) {
   const int64_t max_keys = static_cast<int64_t>(p.max_pages) * p.block_size;
   int s = 1;
@@ -746,15 +747,17 @@ template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_s
 }
 
 // Whether a call takes the wide kernel (128 rows a CTA on the 5th-generation tensor cores) rather than blocks of 16 rows of
-// this one. Measured on B200, head_dim 128, group 4, this kernel against the wide one, us:
-//   16-bit cache, 32 sequences of up to 2048 keys: 64 rows 80 / 87, 128 rows 151 / 99
-//   16-bit cache, 8 sequences of up to 16384 keys: 64 rows 145 / 97, 256 rows 410 / 116
-//   8-bit cache,  32 sequences of up to 2048 keys: 64 rows 74 / 133, 128 rows 132 / 152
-//   8-bit cache,  8 sequences of up to 16384 keys: 64 rows 107 / 146, 256 rows 351 / 228
-// (the wide kernel has to convert 8-bit tiles through shared memory; many keys let its roles run undisturbed).
+// this one. Measured on B200, head_dim 128, group 4, this kernel / the wide one, us, for ragged batches of (sequences x keys):
+//   16-bit cache, 64 rows:  32 x 2048  80 /  87, 32 x 4096 182 / 116, 8 x 16384 144 /  96
+//   16-bit cache, 128 rows: 32 x 2048 151 / 100, 32 x 4096 225 / 122, 8 x 16384 271 / 109
+//   8-bit cache,  64 rows:  32 x 2048  74 / 133, 32 x 4096 139 / 188, 8 x 16384 106 / 149
+//   8-bit cache,  128 rows: 32 x 2048 132 / 157, 32 x 4096 241 / 228, 8 x 16384 213 / 150
+//   8-bit cache,  256 rows: 4 x 2048   61 /  46, 8 x 16384 351 / 228
+// (8-bit tiles pass through shared memory twice there; long tables let its roles run undisturbed).
 bool prefers_wide(const CacheAttnParams &p, int ct) {
-  if (ct == kE4M3 || ct == kI8) return p.rows > 128;
-  return p.rows > 64 || (p.rows > 32 && static_cast<int64_t>(p.max_pages) * p.block_size > 2 * kFewKeys);
+  const bool many_keys = static_cast<int64_t>(p.max_pages) * p.block_size > kFewKeys;
+  const int few_rows = ct == kE4M3 || ct == kI8 ? 64 : 32;
+  return p.rows > (many_keys ? few_rows : 2 * few_rows);
 }
 
 // Checks a call and fills `p` (all but the workspace) and *ct; *launch = false where there is nothing to do.

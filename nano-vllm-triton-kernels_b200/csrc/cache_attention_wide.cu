@@ -9,8 +9,8 @@
 //     P read from TMEM, where it overwrites its S;
 //   * warps 0-3, one thread per row: the running softmax. The maximum that weights refer to moves only when a row exceeds
 //     it by 2^8 (weights stay below 2^9, in range for fp16), so O is rarely rescaled; the sums are fp32.
-// Two CTAs share an SM (113 KB of shared memory and 256 TMEM columns each): the one computes while the other waits. The
-// grid is what the GPU holds at once, and each CTA takes an even share of the batch's tiles (cache_attention.cuh); the
+// 16-bit caches: two CTAs share an SM (113 KB of shared memory and 256 TMEM columns each), the one computes while the other
+// waits; 8-bit caches: one, with deeper rings. The grid is what the GPU holds at once, and each CTA takes an even share of the batch's tiles (cache_attention.cuh); the
 // roles walk the CTA's segments independently, so the loads of a segment start while the one before is finished.
 // Waits are bounded; a CTA that gives up sets NVB200_STATUS_WAIT_TIMEOUT and lets its copies land.
 #include <algorithm>
@@ -52,7 +52,8 @@ template <int CT, int D> struct Wide {
   static constexpr int kOffV = kOffK + NK * kOpBytes;
   static constexpr int kOffRaw = kOffV + NV * kOpBytes;
   static constexpr int kOffRawScale = kOffRaw + NR * 2 * kRawBytes;          // [NR][2][64] fp32: K scales, V scales
-  static constexpr int kOffScale = kOffRawScale + NR * 2 * kTileKeys * 4;  // [kSlots] of [3][64] fp32 (K scales, V scales, log2 bounds), 2 x largest and 2 x smallest bound
+  // [kSlots] of [3][64] fp32 (K scales, V scales, log2 bounds), 2 x largest and 2 x smallest bound
+  static constexpr int kOffScale = kOffRawScale + NR * 2 * kTileKeys * 4;
   static constexpr int kSlotBytes = kQuant ? 3 * kTileKeys * 4 + 16 : 0;
   static constexpr int kOffHdr = kOffScale + kSlots * kSlotBytes;
   static_assert(kOffHdr + 1024 <= kSmem, "a CTA's shared memory");
@@ -870,7 +871,7 @@ bool make_cache_map(CUtensorMap *map, const void *base, const CacheAttnParams &p
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Rows of a unit. 8-bit caches come with more than 128 rows only.
+// Rows of a unit. 8-bit caches come here with more than 64 rows only.
 int wide_rows(const CacheAttnParams &p, int ct) { return p.rows <= 64 && ct != kE4M3 && ct != kI8 ? 64 : 128; }
 
 // CTAs: as many as run at once, fewer where the longest possible sequences could not feed them.
