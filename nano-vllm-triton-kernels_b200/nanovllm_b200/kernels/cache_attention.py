@@ -83,7 +83,7 @@ def _run(what, q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table
                  "draft_lens must be int32 [B] on q's device")
         draft_lens = draft_lens if draft_lens.is_contiguous() else draft_lens.contiguous()
         drafts = draft_lens.data_ptr()
-    out = torch.empty((B, n, hq, d), dtype=q.dtype, device=dev)
+    out = q.new_empty((B, n, hq, d))
     if B == 0 or n == 0:
         return out
     sk = k_cache.stride()
