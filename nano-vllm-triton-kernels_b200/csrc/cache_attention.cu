@@ -48,6 +48,18 @@ template <int CT> NVB200_DEVICE void mma_ct(float (&d)[4], const uint32_t (&a)[4
   else mma_16816_f16(d, a, b0, b1);
 }
 
+// (a, b) * (x, y) and (a, b) + (x, y), each lane rounded as the scalar operation, in one instruction.
+NVB200_DEVICE void mul2(float &a, float &b, float x, float y) {
+  asm("{\n .reg .b64 p, q;\n mov.b64 p, {%0, %1};\n mov.b64 q, {%2, %3};\n mul.rn.f32x2 p, p, q;\n mov.b64 {%0, %1}, p;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y));
+}
+NVB200_DEVICE void add2(float &a, float &b, float x, float y) {
+  asm("{\n .reg .b64 p, q;\n mov.b64 p, {%0, %1};\n mov.b64 q, {%2, %3};\n add.rn.f32x2 p, p, q;\n mov.b64 {%0, %1}, p;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y));
+}
+
 // Transposes an 8 x 8 matrix of 16-bit elements held two to a lane.
 NVB200_DEVICE uint32_t movmatrix_trans(uint32_t a) {
   uint32_t r;
@@ -194,14 +206,29 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        float &x0 = s[kb][n][2 * i], &x1 = s[kb][n][2 * i + 1];
+        mul2(x0, x1, q.rs[n][0], q.rs[n][1]);
+        if constexpr (C::kQuant) mul2(x0, x1, ks, ks);
+      }
+    }
+  }
+  bool bad = false;  // a row scale of V is not finite, and a row may not see its key
+  if (edge) {
+    bool odd = false;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float &x = s[kb][n][2 * i + e];
-          x = C::kQuant ? x * q.rs[n][e] * ks : x * q.rs[n][e];
-          if (edge && !((see[n][e] >> key) & 1u)) x = -INFINITY;
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (C::kQuant) odd |= !(vs[kb][i] <= 3.402823466e38f);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!((see[n][e] >> (16 * kb + 8 * i + g)) & 1u)) s[kb][n][2 * i + e] = -INFINITY;
         }
       }
     }
+    bad = __any_sync(0xffffffffu, odd);
   }
   uint32_t pb[KB][NT][2];  // weights as the second operand of V^T P^T
 #pragma unroll
@@ -232,26 +259,38 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<
       st.m[n][e] = mt;
       st.l[n][e] *= al;
     }
+    float w[KB][2][2];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float w[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x = s[kb][n][2 * i + e];
-          w[e] = ex2_approx_ftz(x - mu[e]);
-          st.l[n][e] += w[e];
-          if constexpr (C::kQuant) w[e] = x == -INFINITY ? 0.f : w[e] * vs[kb][i] * cw[e];  // (vs may be NaN)
+        float &w0 = w[kb][i][0], &w1 = w[kb][i][1];
+        w0 = s[kb][n][2 * i], w1 = s[kb][n][2 * i + 1];
+        add2(w0, w1, -mu[0], -mu[1]);
+        w0 = ex2_approx_ftz(w0), w1 = ex2_approx_ftz(w1);
+        add2(st.l[n][0], st.l[n][1], w0, w1);
+        if constexpr (C::kQuant) {
+          mul2(w0, w1, vs[kb][i], vs[kb][i]);
+          mul2(w0, w1, cw[0], cw[1]);
         }
-        pb[kb][n][i] = movmatrix_trans(C::kBf16Mma ? pack_bf16x2(w[0], w[1]) : pack_f16x2(w[0], w[1]));
       }
+    }
+    if (C::kQuant && bad) {
+#pragma unroll
+      for (int k = 0; k < KB * 4; ++k)
+        if (s[k / 4][n][k % 4] == -INFINITY) w[k / 4][k % 4 / 2][k % 2] = 0.f;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        pb[kb][n][i] = movmatrix_trans(C::kBf16Mma ? pack_bf16x2(w[kb][i][0], w[kb][i][1]) : pack_f16x2(w[kb][i][0], w[kb][i][1]));
     }
     if (__any_sync(0xffffffffu, ao[0] != 1.f || ao[1] != 1.f)) {
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
-        st.o[c][n][0] *= ao[0], st.o[c][n][1] *= ao[1];
-        st.o[c][n][2] *= ao[0], st.o[c][n][3] *= ao[1];
+        mul2(st.o[c][n][0], st.o[c][n][1], ao[0], ao[1]);
+        mul2(st.o[c][n][2], st.o[c][n][3], ao[0], ao[1]);
       }
     }
   }
