@@ -83,17 +83,30 @@ template <int CT, int D, int NT> struct Geometry {
   static constexpr int kKvBytes = kTile * kRowBytes;
   static constexpr int kScaleBytes = CacheType<CT>::kQuant ? 2 * kTile * 4 : 0;
   static constexpr int kStageBytes = 2 * kKvBytes + kScaleBytes + 128;  // a multiple of 128
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kStride = D + 4;  // floats per record: o[D], m, l, M, flag
-  static constexpr int kRecords = kWarps * kRows * kStride * 4;
-  static constexpr int kPartials = (kMaxSplits + kRows - 1) * kStride * 4;  // splits * ceil(kRows / splits) records
-  static constexpr int kRowBytesOut = kRows * 16;  // merged m, l, M, flag per row
-  static constexpr int kSmem = kRing + kRecords + kRowBytesOut;
-  static_assert(kPartials <= kRing, "a cluster's records take the ring's place");
-  static constexpr int kCtasPerSm = 228 * 1024 / (kSmem + 1024) >= 3 ? 3 : 2;
   // Physical 16-byte chunk of logical chunk c of row r: the 8 rows of an 8 x 16-byte matrix at one logical chunk fall
   // in distinct bank groups (two 64-byte rows share a 128-byte line, so their swizzle steps every second row).
   static NVB200_DEVICE int chunk(int r, int c) { return kRowBytes == 64 ? c ^ ((r >> 1) & 3) : c ^ (r & 7); }
+};
+
+// What the two forms of the kernel lay out differently. The warps' records of their partial results lie, in the cluster
+// form, where a CTA has one segment, in the warps' own rings; in the even-share form, where the next segment's tiles are
+// landing there already, beside them. The saving lets three CTAs of the cluster form share an SM for at most 8 rows (256
+// sequences of 300 keys, e4m3: 60 -> 49 us; six warps a CTA in the same memory: 56 us).
+template <int CT, int D, int NT, bool CLUSTER> struct Form {
+  using G = Geometry<CT, D, NT>;
+  static constexpr int kWarpRing = G::kStages * G::kStageBytes;
+  static constexpr int kRing = kWarps * kWarpRing;
+  static constexpr int kRecord = G::kRows * G::kStride * 4;
+  static constexpr int kRecords = CLUSTER ? 0 : kRing;                     // where the records lie
+  static constexpr int kRecordStep = (CLUSTER ? kWarpRing : kRecord) / 4;  // floats from one warp's to the next
+  static_assert(!CLUSTER || kRecord <= kWarpRing, "a warp's record takes its ring's place");
+  // Cluster form: the records that a CTA receives, splits * ceil(kRows / splits) rows.
+  static constexpr int kReceived = kRing;
+  static constexpr int kRowsAt = kRing + (CLUSTER ? (kMaxSplits + G::kRows - 1) * G::kStride * 4 : kWarps * kRecord);
+  static constexpr int kSmem = kRowsAt + G::kRows * 16;  // merged m, l, M, flag per row
+  static constexpr int kCtasPerSm = NT == 1 && 228 * 1024 / (kSmem + 1024) >= 3 ? 3 : 2;
+  static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 // One warp's softmax state. The products are S^T = K Q^T and O^T = V^T P^T: the keys (and the output's columns) fill the
@@ -331,18 +344,19 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<
 // CLUSTER: the CTAs of a cluster split one unit's keys evenly and merge through distributed shared memory (grid: splits,
 // units of a sequence, batch). Else: even shares of the whole batch (cache_attention.cuh).
 template <int CT, int D, int NT, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
+__global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm)
     cache_attention_kernel(const __grid_constant__ CacheAttnParams p) {
   using G = Geometry<CT, D, NT>;
+  using F = Form<CT, D, NT, CLUSTER>;
   using C = CacheType<CT>;
   launch_dependents();     // a dependent launched early waits for this grid before reading its output
   grid_dependency_wait();  // this grid may itself have been launched early
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  const uint32_t wring = smem_addr(smem) + warp * (G::kStages * G::kStageBytes);
-  float *rec = reinterpret_cast<float *>(smem + G::kRing);  // [kWarps][kRows][kStride]
-  float4 *row_s = reinterpret_cast<float4 *>(smem + G::kRing + G::kRecords);  // [kRows]
+  const uint32_t wring = smem_addr(smem) + warp * F::kWarpRing;
+  float *rec = reinterpret_cast<float *>(smem + F::kRecords);  // kRecordStep apart, [kRows][kStride] each
+  float4 *row_s = reinterpret_cast<float4 *>(smem + F::kRowsAt);  // [kRows]
 
   Segment seg;
   int u1, T = 0, ctas = 0;
@@ -374,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
   }
   const bool masked = p.mask != nullptr || p.causal;
 
-  // The warp's issue cursor: it takes every 4th tile of each segment, and runs ahead of the tiles being folded, past the
+  // The warp's issue cursor: it takes every kWarps-th tile of each segment, and runs ahead of the tiles being folded, past the
   // segment's end.
   Segment is = seg;
   int ik = warp, next_blk = -1;
@@ -598,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float *w = rec + (warp * G::kRows + 8 * n + 2 * t + e) * G::kStride;
+        float *w = rec + warp * F::kRecordStep + (8 * n + 2 * t + e) * G::kStride;
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
           if constexpr (C::kQuant) {
@@ -636,26 +650,25 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
         to[2] = static_cast<uint16_t>(hi), to[3] = static_cast<uint16_t>(hi >> 16);
       }
     };
-    merge_rows(rec, nrows, G::kStride, kWarps, G::kRows * G::kStride);
+    merge_rows(rec, nrows, G::kStride, kWarps, F::kRecordStep);
 
     if constexpr (CLUSTER) {
       if (p.splits == 1) {
         for (int e = tid; e < nrows * kPer; e += kThreads) {
           const int r = e / kPer, d = e % kPer * 4;
-          write(r, d, row4(rec + r * G::kStride, d, kWarps, G::kRows * G::kStride), row_s[r]);
+          write(r, d, row4(rec + r * G::kStride, d, kWarps, F::kRecordStep), row_s[r]);
         }
         return;
       }
-      // Row r is finished by CTA r mod splits: every CTA sends its merged record there, into the ring's place (the first
-      // barrier: the receiver's ring is no longer in use; the second: every record has arrived).
+      // Row r is finished by CTA r mod splits: every CTA sends its merged record there (the first barrier: every CTA of the
+      // cluster has started; the second: every record has arrived).
       const int rank = static_cast<int>(cta_rank_in_cluster());
-      float *part = reinterpret_cast<float *>(smem);  // [rows finished here][splits][kStride]
-      cp_async_wait<0>();
+      float *part = reinterpret_cast<float *>(smem + F::kReceived);  // [rows finished here][splits][kStride]
       cluster_arrive();
       cluster_wait();
       for (int e = tid; e < nrows * kPer; e += kThreads) {
         const int r = e / kPer, d = e % kPer * 4;
-        const float4 o = row4(rec + r * G::kStride, d, kWarps, G::kRows * G::kStride);
+        const float4 o = row4(rec + r * G::kStride, d, kWarps, F::kRecordStep);
         const uint32_t to = map_shared_to(smem_addr(part + ((r / p.splits) * p.splits + rank) * G::kStride), r % p.splits);
         st_cluster_v4(to + d * 4, o);
         if (d == 0) st_cluster_v4(to + D * 4, row_s[r]);
@@ -674,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, Geometry<CT, D, NT>::kCtasPerSm)
       float *out = p.records + static_cast<int64_t>(record_slot(blockIdx.x, seg.unit_u, T, ctas)) * G::kRows * G::kStride;
       for (int e = tid; e < nrows * kPer; e += kThreads) {
         const int r = e / kPer, d = e % kPer * 4;
-        const float4 o = row4(rec + r * G::kStride, d, kWarps, G::kRows * G::kStride);
+        const float4 o = row4(rec + r * G::kStride, d, kWarps, F::kRecordStep);
         if (whole) {
           write(r, d, o, row_s[r]);
         } else {
@@ -704,23 +717,26 @@ template <typename Kernel> int allow_smem(Kernel kernel, int bytes, std::atomic<
   return NVB200_OK;
 }
 
-// Largest power of two of CTAs per cluster that the longest possible sequence feeds with a tile for every other warp, while
-// the clusters fit on the GPU at once (one sequence of 611 keys: 4 CTAs 8.0 us, 8 CTAs 7.0 us).
-int cluster_splits(const CacheAttnParams &p, int64_t units, int tile, int ctas_per_sm) {
+// CTAs per cluster, a power of two: as many as the longest possible sequence feeds with a tile per warp, while the clusters
+// fit on the GPU at once (one sequence of 611 keys: 4 CTAs 8.0 us, 8 CTAs 7.0 us); 1 for up to four tiles a warp, which take
+// no longer than the start and the barriers of a cluster (42 x 4 heads of 59 keys in tables of 256: 6.2 against 8.3 us).
+int cluster_splits(const CacheAttnParams &p, int64_t units, int cta_keys, int ctas_per_sm) {
   const int64_t max_keys = static_cast<int64_t>(p.max_pages) * p.block_size;
+  if (max_keys < 4 * cta_keys) return 1;
   int s = 1;
-  while (s < kMaxSplits && 2 * s * units <= static_cast<int64_t>(ctas_per_sm) * sm_count() && s * kWarps * tile <= max_keys)
+  while (s < kMaxSplits && 2 * s * units <= static_cast<int64_t>(ctas_per_sm) * sm_count() && s * cta_keys <= max_keys)
     s *= 2;
   return s;
 }
 
 struct NarrowShape {
   int64_t units;  // of a sequence
-  int tile, rows, ctas_per_sm;
+  int tile, rows, ctas_per_sm;  // (of the even-share form)
 };
 template <int CT, int D, int NT> NarrowShape shape_of(const CacheAttnParams &p) {
   using G = Geometry<CT, D, NT>;
-  return {static_cast<int64_t>(p.hkv) * ((p.rows + G::kRows - 1) / G::kRows), G::kTile, G::kRows, G::kCtasPerSm};
+  return {static_cast<int64_t>(p.hkv) * ((p.rows + G::kRows - 1) / G::kRows), G::kTile, G::kRows,
+          Form<CT, D, NT, false>::kCtasPerSm};
 }
 
 // The one place that picks a kernel: f(cache type, head_dim, row tiles of 8) as integral constants. More than 16 rows are
@@ -767,22 +783,26 @@ int narrow_grid(const CacheAttnParams &p, const NarrowShape &n, int num_splits) 
 
 template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_splits, void *workspace, cudaStream_t s) {
   using G = Geometry<CT, D, NT>;
+  using Share = Form<CT, D, NT, false>;
+  using Cluster = Form<CT, D, NT, true>;
   const NarrowShape n = shape_of<CT, D, NT>(p);
   const int grid = workspace ? narrow_grid(p, n, num_splits) : 0;
   if (grid > 0) {
     place_workspace(p, workspace, grid);
     static std::atomic<uint64_t> ready{0};  // bit: device whose shared-memory limit is set
-    if (int rc = allow_smem(cache_attention_kernel<CT, D, NT, false>, G::kSmem, ready)) return rc;
-    if (int rc = launch_ex(cache_attention_kernel<CT, D, NT, false>, dim3(grid), dim3(kThreads), G::kSmem, s, 1, false, p))
+    if (int rc = allow_smem(cache_attention_kernel<CT, D, NT, false>, Share::kSmem, ready)) return rc;
+    if (int rc = launch_ex(cache_attention_kernel<CT, D, NT, false>, dim3(grid), dim3(kThreads), Share::kSmem, s, 1,
+                           false, p))
       return rc;
     return launch_cache_attention_merge(p, CT, D, G::kRows, grid, s);
   }
   static std::atomic<uint64_t> ready{0};
-  if (int rc = allow_smem(cache_attention_kernel<CT, D, NT, true>, G::kSmem, ready)) return rc;
+  if (int rc = allow_smem(cache_attention_kernel<CT, D, NT, true>, Cluster::kSmem, ready)) return rc;
   if (n.units > 65535 || p.batch > 65535) return NVB200_ERR_UNSUPPORTED;
-  p.splits = num_splits > 0 ? num_splits : cluster_splits(p, n.units * p.batch, n.tile, n.ctas_per_sm);
+  p.splits = num_splits > 0 ? num_splits
+                            : cluster_splits(p, n.units * p.batch, kWarps * G::kTile, Cluster::kCtasPerSm);
   return launch_ex(cache_attention_kernel<CT, D, NT, true>, dim3(p.splits, static_cast<unsigned>(n.units), p.batch),
-                   dim3(kThreads), G::kSmem, s, p.splits, false, p);
+                   dim3(kThreads), Cluster::kSmem, s, p.splits, false, p);
 }
 
 // Whether a call takes the wide kernel (128 rows a CTA on the 5th-generation tensor cores) rather than blocks of 16 rows of
