@@ -358,14 +358,46 @@ __global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm
   float *rec = reinterpret_cast<float *>(smem + F::kRecords);  // kRecordStep apart, [kRows][kStride] each
   float4 *row_s = reinterpret_cast<float4 *>(smem + F::kRowsAt);  // [kRows]
 
+  // The unit's query rows as the lanes take them (row g of each row tile), from row0 of KV head h.
+  uint32_t wq[NT][D / 16][2];
+  auto load_q = [&](int b, int h, int row0) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = row0 + 8 * n + g, qi = r / p.group;
+      const uint16_t *row = r < p.rows ? static_cast<const uint16_t *>(p.q) + b * p.q_batch_stride +
+                                             qi * p.q_token_stride +
+                                             static_cast<int64_t>(h * p.group + r - qi * p.group) * p.q_head_stride
+                                       : nullptr;
+      // Lane t's elements: 16-bit caches 16 ks + 2 t, + 1, + 8, + 9; 8-bit caches 16 ks + 4 t .. + 3.
+      uint32_t(&w)[D / 16][2] = wq[n];
+      const bool pairs = (reinterpret_cast<uintptr_t>(row) & 7) == 0;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const int d0 = 16 * ks + (C::kQuant ? 4 * t : 2 * t), d1 = C::kQuant ? d0 + 2 : d0 + 8;
+        w[ks][0] = w[ks][1] = 0u;
+        if (row && pairs) {
+          w[ks][0] = __ldg(reinterpret_cast<const uint32_t *>(row + d0));
+          w[ks][1] = __ldg(reinterpret_cast<const uint32_t *>(row + d1));
+        } else if (row) {
+          w[ks][0] = static_cast<uint32_t>(__ldg(row + d0)) | static_cast<uint32_t>(__ldg(row + d0 + 1)) << 16;
+          w[ks][1] = static_cast<uint32_t>(__ldg(row + d1)) | static_cast<uint32_t>(__ldg(row + d1 + 1)) << 16;
+        }
+      }
+    }
+  };
+
   Segment seg;
   int u1, T = 0, ctas = 0;
   if constexpr (CLUSTER) {
     const int row_blocks = (p.rows + G::kRows - 1) / G::kRows;
     const int b = blockIdx.z, rank = p.splits > 1 ? static_cast<int>(cta_rank_in_cluster()) : 0;
+    const int h = blockIdx.y / row_blocks, block = blockIdx.y - h * row_blocks;
+    // The queries' loads and the block table's first lines do not wait for the length, nor behind the keys' loads.
+    load_q(b, h, block * G::kRows);
+    if (p.block_table && 32 * lane < p.max_pages)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.block_table + b * p.bt_stride + 32 * lane));
     seg.b = b;
     seg.s = seq_info(p, b, G::kTile, G::kRows, tid == 0 && rank == 0 && blockIdx.y == 0);
-    const int h = blockIdx.y / row_blocks, block = blockIdx.y - h * row_blocks;
     const int tiles = block < seg.s.blocks ? seg.s.tiles : 0;  // else only padding rows
     seg.s.blocks = row_blocks;
     seg.unit = blockIdx.y;
@@ -386,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm
     if (tid == 0) write_cut(p, blockIdx.x, seg, T, ctas);
     if (!work) return;
   }
-  const bool masked = p.mask != nullptr || p.causal;
+  const bool masked = p.mask != nullptr || (p.causal && p.n > 1);  // (one token of a chain sees every key)
 
   // The warp's issue cursor: it takes every kWarps-th tile of each segment, and runs ahead of the tiles being folded, past the
   // segment's end.
@@ -489,27 +521,10 @@ __global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm
     // (bf16's range does not fit fp16; elements below 2^-27 of the largest lose bits, fewer than the fp32 sum would). rs:
     // what the scores of rows 2 t and 2 t + 1 are multiplied by.
     QueryFrags<D, NT> q;
+    if constexpr (!CLUSTER) load_q(b, h, row0);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = row0 + 8 * n + g, qi = r / p.group;
-      const uint16_t *row = r < p.rows ? static_cast<const uint16_t *>(p.q) + b * p.q_batch_stride +
-                                             qi * p.q_token_stride +
-                                             static_cast<int64_t>(h * p.group + r - qi * p.group) * p.q_head_stride
-                                       : nullptr;
-      // Lane t's elements: 16-bit caches 16 ks + 2 t, + 1, + 8, + 9; 8-bit caches 16 ks + 4 t .. + 3.
-      uint32_t w[D / 16][2];
-      const bool pairs = (reinterpret_cast<uintptr_t>(row) & 7) == 0;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const int d0 = 16 * ks + (C::kQuant ? 4 * t : 2 * t), d1 = C::kQuant ? d0 + 2 : d0 + 8;
-        w[ks][0] = w[ks][1] = 0u;
-        if (row && pairs) {
-          w[ks][0] = __ldg(reinterpret_cast<const uint32_t *>(row + d0)), w[ks][1] = __ldg(reinterpret_cast<const uint32_t *>(row + d1));
-        } else if (row) {
-          w[ks][0] = static_cast<uint32_t>(__ldg(row + d0)) | static_cast<uint32_t>(__ldg(row + d0 + 1)) << 16;
-          w[ks][1] = static_cast<uint32_t>(__ldg(row + d1)) | static_cast<uint32_t>(__ldg(row + d1 + 1)) << 16;
-        }
-      }
+      uint32_t(&w)[D / 16][2] = wq[n];
       float f = p.scale_log2;
       if constexpr (C::kQuant) {
         uint32_t am = 0;  // largest magnitude, as 16-bit patterns (they order like the values)
@@ -557,7 +572,11 @@ __global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm
       constexpr uint32_t kAll = G::kTile == 32 ? 0xFFFFFFFFu : (1u << (G::kTile & 31)) - 1u;
       const bool edge = live != kAll || j0 + G::kTile > open;
       uint32_t see[NT][2];
-      if (edge) {
+      if (edge && (!masked || j0 + G::kTile <= open)) {
+        // Rows of padding tokens included: they are written as zeros whatever they sum.
+#pragma unroll
+        for (int n = 0; n < NT; ++n) see[n][0] = see[n][1] = live;
+      } else if (edge) {
         // Keys below `open` are seen, then new token rel0 + k at key k.
         const int rel0 = j0 - ctx;
         const uint32_t before = open > j0 ? (open - j0 >= 32 ? 0xFFFFFFFFu : (1u << (open - j0)) - 1u) : 0u;
@@ -572,9 +591,7 @@ __global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm
               last_qi = qi;
               word = 0;
               if (qi < drafts && row0 + 8 * n + r < p.rows) {
-                if (j0 + G::kTile <= open || !masked) {
-                  word = 0xFFFFFFFFu;
-                } else if (p.mask) {
+                if (p.mask) {
                   const int x = rel0 + lane;
                   const bool is = x >= 0 && x < drafts &&
                                   __ldg(p.mask + b * p.mask_batch_stride + qi * p.mask_row_stride + x) != 0;

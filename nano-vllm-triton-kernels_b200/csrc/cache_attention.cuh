@@ -270,7 +270,7 @@ NVB200_DEVICE int page_of(const CacheAttnParams &p, int j) {
 // row may not see them); a row that does see one gets it here, where it decides column d whatever its weight. y: the
 // row's output without them.
 template <int CT>
-NVB200_DEVICE float add_nonfinite(const CacheAttnParams &p, const int32_t *bt, int b, int h, int qi, int d, int ctx, int L,
+__device__ __noinline__ float add_nonfinite(const CacheAttnParams &p, const int32_t *bt, int b, int h, int qi, int d, int ctx, int L,
                                   int drafts, float y) {
   for (int k = 0; k < drafts; ++k) {
     const int j = ctx + k;
