@@ -131,11 +131,11 @@ template <int D, int NT> struct QueryFrags {
   float rs[NT][2];
 };
 
-// Replaces every infinity and NaN of the V tile by zero; true if there were any (in any lane).
-template <int CT, int D, int NT> NVB200_DEVICE bool clean_v_tile(uint32_t kt, int lane) {
+// Replaces every infinity and NaN of the V tile's rows from `first` on by zero; true if there were any (in any lane).
+template <int CT, int D, int NT> NVB200_DEVICE bool clean_v_tile(uint32_t kt, int first, int lane) {
   using G = Geometry<CT, D, NT>;
   uint32_t found = 0;
-  for (int o = lane * 16; o < G::kKvBytes; o += 512) {
+  for (int o = first * G::kRowBytes + lane * 16; o < G::kKvBytes; o += 512) {
     uint4 u = ld_shared_v4(kt + G::kKvBytes + o);
     uint32_t *w = &u.x;
     uint32_t here = 0;
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm
         // 0 * inf is NaN in the matrix instruction, so where a row may not see a key of this tile, V must be finite. (Of the
         // 8-bit types e4m3 has a NaN, which the quantiser never writes; a NaN scale meets selected weights only.)
         if constexpr (CT != kI8) {
-          if (j0 + G::kTile > open && (p.mask ? drafts > 0 : drafts > 1)) dirty |= clean_v_tile<CT, D, NT>(kt, lane);
+          if (j0 + G::kTile > open && (p.mask ? drafts > 0 : drafts > 1)) dirty |= clean_v_tile<CT, D, NT>(kt, max(0, open - j0), lane);
         }
       }
       fold_tile<CT, D, NT>(st, kt, q, lane, edge, see);
@@ -897,7 +897,7 @@ extern "C" int64_t nvb200_cache_attention_workspace_size(const nvb200_cache_atte
   bool launch = false;
   if (prepare_attention(a, p, &ct, &launch) != NVB200_OK) return -1;
   if (!launch) return 0;
-  if (prefers_wide(p, ct) && a->num_splits == 0 && wide_takes(p, ct)) return wide_workspace_bytes(p, ct, a->head_dim);
+  if (prefers_wide(p, ct) && a->num_splits == 0 && wide_takes(p)) return wide_workspace_bytes(p, ct, a->head_dim);
   const NarrowShape n = narrow_shape(p, ct, a->head_dim);
   return even_share_bytes(narrow_grid(p, n, a->num_splits), n.rows, a->head_dim);
 }
@@ -915,7 +915,7 @@ extern "C" int nvb200_cache_attention(const nvb200_cache_attention_args *a, void
   if (workspace && workspace_bytes < need) return NVB200_ERR_ARG;
   if (need == 0) workspace = nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (prefers_wide(p, ct) && a->num_splits == 0 && workspace && wide_takes(p, ct)) {
+  if (prefers_wide(p, ct) && a->num_splits == 0 && workspace && wide_takes(p)) {
     const int rc = launch_cache_attention_wide(p, ct, a->head_dim, workspace, s);
     if (rc != NVB200_ERR_UNSUPPORTED) return rc;
     workspace = nullptr;  // sized for the other kernel: the cluster form needs none

@@ -129,10 +129,7 @@ NVB200_DEVICE void mul2(float &a, float &b, float c, float d) {
 // Swizzled position of 16-byte chunk c (0-7) of 128-byte row r in a tile of such rows.
 NVB200_DEVICE uint32_t swz128(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
 
-// REP = 2 (at most 64 rows): every row twice in the 128 lanes of a tile, lane r taking keys 0-31 of each tile and lane 64 +
-// r keys 32-63, as if they were two shares of the keys; the tile's products cost what they cost for 128 rows, but a softmax
-// thread has half the work.
-template <int CT, int D, int REP>
+template <int CT, int D>
 __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
     cache_attention_wide_kernel(const __grid_constant__ WideParams wp, const __grid_constant__ WideMaps maps) {
   using W = Wide<CT, D>;
@@ -142,23 +139,22 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
   extern __shared__ __align__(1024) uint8_t smem[];
   const CacheAttnParams &p = wp.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kUnitRows = kTileRows / REP;  // rows of a unit
   const uint32_t base = smem_addr(smem);
-  const int T = total_work(p, kTileKeys, kUnitRows);  // by every warp
+  const int T = total_work(p, kTileKeys, kTileRows);  // by every warp
   const int G = active_ctas(T, gridDim.x, kMinTiles);
-  zero_uncovered_rows(p, D, kTileKeys, kUnitRows, blockIdx.x, gridDim.x, tid, W::kThreads);
+  zero_uncovered_rows(p, D, kTileKeys, kTileRows, blockIdx.x, gridDim.x, tid, W::kThreads);
   const bool work = T > 0 && static_cast<int>(blockIdx.x) < G;
   const int u0 = work ? range_start(blockIdx.x, T, G) : 0, u1 = work ? range_start(blockIdx.x + 1, T, G) : 0;
   Segment seg;
   seg.n = 0;
-  if (work) seg = find_segment(p, u0, u1, kTileKeys, kUnitRows);
+  if (work) seg = find_segment(p, u0, u1, kTileKeys, kTileRows);
   if (tid == 0) write_cut(p, blockIdx.x, seg, T, G);
   if (!work) return;
-  auto next = [&]() { next_segment(seg, p, u1, kTileKeys, kUnitRows); };
+  auto next = [&]() { next_segment(seg, p, u1, kTileKeys, kTileRows); };
 
   const uint32_t hdr = base + W::kOffHdr;
   const uint32_t b_kfull = hdr, b_kempty = hdr + 32, b_vfull = hdr + 64, b_vempty = hdr + 96;  // up to 4 each
-  const uint32_t b_sfull = hdr + 128, b_pready = hdr + 144, b_q = hdr + 168, b_meet = hdr + 176;
+  const uint32_t b_sfull = hdr + 128, b_pready = hdr + 144, b_q = hdr + 168;
   const uint32_t b_pv = hdr + 184;  // 2, like b_sfull and b_pready by tile parity: the softmax may be two P V ahead of one
   const uint32_t b_rfull = hdr + 200, b_rempty = hdr + 264;              // up to 8 each
   const uint32_t live_slot = hdr + 328, raw_live = hdr + 392;            // 64-bit words: up to 8 each
@@ -169,7 +165,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
     for (int i = 0; i < W::NK; ++i) mbar_init(b_kfull + 8 * i, W::kQuant ? W::kConvWarps : 1), mbar_init(b_kempty + 8 * i, 1);
     for (int i = 0; i < W::NV; ++i) mbar_init(b_vfull + 8 * i, W::kQuant ? W::kConvWarps : 1), mbar_init(b_vempty + 8 * i, 1);
     for (int i = 0; i < 2; ++i) mbar_init(b_sfull + 8 * i, 2), mbar_init(b_pready + 8 * i, 4), mbar_init(b_pv + 8 * i, 1);
-    mbar_init(b_q, 4), mbar_init(b_meet, 4);
+    mbar_init(b_q, 4);
     for (int i = 0; i < W::NR; ++i) mbar_init(b_rfull + 8 * i, 1), mbar_init(b_rempty + 8 * i, W::kConvWarps);
     st_shared_u32(failed, 0u), st_shared_u32(dirty, 0u);
     fence_mbar_init();
@@ -382,9 +378,9 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
       constexpr int kChunks = D / 16;            // 16-byte chunks of a raw row
       constexpr int kRowsPer = 128 / kChunks;    // rows that the 128 threads cover at a time
       const int r8 = (ct & 7) | (ct >> 3) / kChunks * 8, ch = (ct >> 3) % kChunks;
-      // Converts a raw tile to an operand tile; rows whose bit of `live` is clear become zeros, and with `finite` e4m3's
-      // NaN codes too.
-      auto convert = [&](int src, int dst, unsigned long long live, bool finite) {
+      // Converts a raw tile to an operand tile; rows whose bit of `live` is clear become zeros, and from row `finite` on
+      // e4m3's NaN codes too.
+      auto convert = [&](int src, int dst, unsigned long long live, int finite) {
         uint4 u[kTileKeys / kRowsPer];  // all loads before the first store
 #pragma unroll
         for (int k = 0; k < kTileKeys / kRowsPer; ++k) {
@@ -397,7 +393,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
           const int r = k * kRowsPer + r8;
           if (!((live >> r) & 1ull)) u[k] = make_uint4(0u, 0u, 0u, 0u);
           uint32_t *w = &u[k].x;
-          if (CT == kE4M3 && finite) {
+          if (CT == kE4M3 && r >= finite) {
             uint32_t found = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -422,7 +418,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
         const int st = i % W::NR, slot = i % W::kSlots, sk = i % W::NK;
         if (!wait(b_rfull + 8 * st, (i / W::NR) & 1) || !wait(b_kempty + 8 * sk, ((i / W::NK) & 1) ^ 1)) return false;
         const unsigned long long live = live_of(st);
-        convert(W::kOffRaw + st * 2 * W::kRawBytes, W::kOffK + sk * W::kOpBytes, live, false);
+        convert(W::kOffRaw + st * 2 * W::kRawBytes, W::kOffK + sk * W::kOpBytes, live, kTileKeys);
         if (ct < kTileKeys) {
           // The key's scales; zeros where it is none (its slot of the raw tile was not loaded).
           const bool is = (live >> ct) & 1ull;
@@ -458,7 +454,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
           ok = ok && wait(b_vempty + 8 * sv, ((i / W::NV) & 1) ^ 1);
           if (!ok) break;
           convert(W::kOffRaw + st * 2 * W::kRawBytes + W::kRawBytes, W::kOffV + sv * W::kOpBytes, live_of(st),
-                  hides && first_key() + (t + 1) * kTileKeys > open_below());
+                  hides ? open_below() - (first_key() + t * kTileKeys) : kTileKeys);
           arrive(b_vfull + 8 * sv);
           arrive(b_rempty + 8 * st);
         }
@@ -469,21 +465,15 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
     // ---------------------------------------------------------------- softmax: thread = row
     bool ok = true;
     int i = 0;  // tile of the CTA
-    uint32_t met = 0;
-    auto meet = [&]() {  // a barrier of the four softmax warps, bounded as every wait
-      arrive(b_meet);
-      return wait(b_meet, met++ & 1);
-    };
     for (; seg.n > 0 && ok; next()) {
-    const int b = seg.b, h = seg.unit / seg.s.blocks, row0 = (seg.unit - h * seg.s.blocks) * kUnitRows;
-    const int nrows = min(kUnitRows, p.rows - row0), L = seg.s.L, drafts = seg.s.drafts, ctx = context();
+    const int b = seg.b, h = seg.unit / seg.s.blocks, row0 = (seg.unit - h * seg.s.blocks) * kTileRows;
+    const int nrows = min(kTileRows, p.rows - row0), L = seg.s.L, drafts = seg.s.drafts, ctx = context();
     const int js = first_key(), je = static_cast<int>(end_key()), open = open_below();
     const bool hides = hides_keys();
     const int32_t *bt = table_of();
     float m = -INFINITY, l = 0.f, M = -INFINITY;
-    const int vrow = tid % kUnitRows, r = row0 + vrow, qi_raw = r / p.group;
-    const int qi = vrow < nrows && qi_raw < drafts ? qi_raw : -1;
-    const int col0 = tid / kUnitRows * 32;  // REP = 2: the first of the thread's 32 columns (the same for a whole warp)
+    const int r = row0 + tid, qi_raw = r / p.group;
+    const int qi = tid < nrows && qi_raw < drafts ? qi_raw : -1;
     const bool warp_live = __any_sync(0xffffffffu, qi >= 0);
     // The query row into shared memory (128-byte swizzled rows, two sub-tiles of 64 elements at head_dim 128). 8-bit
     // caches: brought to fp16 by an exact power of two (see cache_attention.cu), which the scores give back.
@@ -589,7 +579,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
           const int sv = i % W::NV;
           ok = wait(b_vfull + 8 * sv, (i / W::NV) & 1);
           if (!ok) break;
-          const bool finite = hides && j0 + kTileKeys > open;
+          const int finite = hides ? open - j0 : kTileKeys;  // rows from here on hold new tokens
           for (int c = tid; c < W::kOpBytes / 16; c += kTileRows) {
             const int row = (c >> 3) & (kTileKeys - 1);
             const uint32_t at = base + W::kOffV + sv * W::kOpBytes + c * 16;
@@ -597,7 +587,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
             uint32_t *w = &u.x, change = 0;
             if (!((row < 32 ? lo >> row : hi >> (row - 32)) & 1u)) {
               u = make_uint4(0u, 0u, 0u, 0u), change = 1;
-            } else if (finite) {
+            } else if (row >= finite) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const uint32_t bad = nonfinite_bits<CT>(w[e]);
@@ -632,12 +622,9 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
           if (qi < 0) see = 0ull;
           see_lo = lo & static_cast<uint32_t>(see), see_hi = hi & static_cast<uint32_t>(see >> 32);
         }
-        // Scores of columns c0 .. c0 + CW before the row's factor rs > 0. 8-bit caches with 128 rows read S twice, 32 columns
-        // at a time (for the maximum, then for the weights): a tile's 64 scores beside three numbers per key do not fit
+        // Scores of columns c0 .. c0 + CW before the row's factor rs > 0. 8-bit caches read S twice, 32 columns at a time (for the maximum, then for the weights): a tile's 64 scores beside three numbers per key do not fit
         // the registers of a thread, and what is spilled goes to the L2, the L1 being all shared memory here.
-        constexpr int CW = W::kQuant || REP == 2 ? 32 : 64;
-        constexpr int kCols = kTileKeys / REP;  // of this thread
-        const int first = REP == 2 ? col0 : 0;
+        constexpr int CW = W::kQuant ? 32 : 64;
         float x[CW];
         auto scores = [&](int c0) {
           if constexpr (CW == 32) tmem_ld32(s_addr + c0, x);
@@ -660,7 +647,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
         };
         float top = -INFINITY;
 #pragma unroll 1
-        for (int c0 = first; c0 < first + kCols; c0 += CW) {
+        for (int c0 = 0; c0 < kTileKeys; c0 += CW) {
           scores(c0);
           float mx = fmax3(top, x[0], x[1]), mx1 = fmaxf(x[2], x[3]);
 #pragma unroll
@@ -683,7 +670,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
             Mt = mt + vhi;
           } else if (edge || __any_sync(0xffffffffu, mt + vhi > M + 8.f || M == -INFINITY)) {
 #pragma unroll 1
-            for (int c0 = first; c0 < first + kCols; c0 += CW) {
+            for (int c0 = 0; c0 < kTileKeys; c0 += CW) {
               scores(c0);
 #pragma unroll
               for (int c = 0; c < CW; c += 4) {
@@ -720,8 +707,8 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
         const float cw = W::kQuant ? ex2_approx_ftz(mu - (M == -INFINITY ? 0.f : M)) : 1.f;
         uint64_t sum0 = 0, sum1 = 0;  // pairs of fp32
 #pragma unroll 1
-        for (int c0 = first; c0 < first + kCols; c0 += CW) {
-          if constexpr (kCols > CW) scores(c0);
+        for (int c0 = 0; c0 < kTileKeys; c0 += CW) {
+          if constexpr (W::kQuant) scores(c0);
 #pragma unroll
           for (int h0 = 0; h0 < CW; h0 += 32) {
             uint32_t pk[16];
@@ -748,10 +735,6 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
             tmem_st16(s_addr + (c0 + h0) / 2, pk);  // over scores that have been read
           }
         }
-        if constexpr (REP == 2) {  // the other lane's columns
-          const uint32_t none[16] = {};
-          tmem_st16(s_addr + (32 - col0) / 2, none);
-        }
         const float2 sum = f32x2_unpack(f32x2_add(sum0, sum1));
         l += sum.x + sum.y;
         tmem_st_wait();
@@ -763,81 +746,41 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
     if (!ok) break;
     tc_fence_after();
 
-    // The rows' results. REP = 2: lane 64 + r's half joins lane r's, through the query rows' shared memory (every product
-    // that reads them is done): first both halves' references and sums, then the upper half's output.
-    float own = 1.f;  // what this lane's O is multiplied by
     if constexpr (!W::kQuant) M = m;
-    if constexpr (REP == 2) {
-      float *x = reinterpret_cast<float *>(smem);
-      x[tid * 4] = m, x[tid * 4 + 1] = l, x[tid * 4 + 2] = M;
-      if (!(ok = meet())) break;
-      const float *y = x + (tid ^ kUnitRows) * 4;
-      const float om = y[0], ol = y[1], oM = y[2];
-      if (!(ok = meet())) break;
-      const float mx = fmaxf(m, om), Mx = fmaxf(M, oM);
-      const float mu = mx == -INFINITY ? 0.f : mx, Mu = Mx == -INFINITY ? 0.f : Mx;
-      own = exp2f(M - Mu);
-      l = l * exp2f(m - mu) + ol * exp2f(om - mu);
-      m = mx, M = Mx;
-      uint8_t *half = smem + vrow * D * 4;
-      if (tid >= kUnitRows) {
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float t[32];
-          tmem_ld32(tmem + lanes + kColO + c, t);
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4 *>(half + (((c + e) / 4) ^ (vrow & 7)) * 16) =
-                make_float4(t[e] * own, t[e + 1] * own, t[e + 2] * own, t[e + 3] * own);
-        }
-      }
-      if (!(ok = meet())) break;
-    }
     const bool whole = seg.n == seg.s.tiles;
     const bool flagged = ld_shared_u32(dirty) != 0u;
-    if (tid < kUnitRows) {
-      const int gq = r - qi_raw * p.group;
-      const float f = l == 0.f ? 0.f : (W::kQuant ? exp2f(M - m) : 1.f) / l;
-      float *rec = p.records + (static_cast<int64_t>(record_slot(blockIdx.x, seg.unit_u, T, G)) * kUnitRows + vrow) * (D + 4);
-      const int64_t row = ((static_cast<int64_t>(b) * p.n + qi_raw) * p.hq + h * p.group + gq) * D;
+    const int gq = r - qi_raw * p.group;
+    const float f = l == 0.f ? 0.f : (W::kQuant ? exp2f(M - m) : 1.f) / l;
+    float *rec = p.records + (static_cast<int64_t>(record_slot(blockIdx.x, seg.unit_u, T, G)) * kTileRows + tid) * (D + 4);
+    const int64_t row = ((static_cast<int64_t>(b) * p.n + qi_raw) * p.hq + h * p.group + gq) * D;
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        float t[32];
-        tmem_ld32(tmem + lanes + kColO + c, t);
-        if constexpr (REP == 2) {
+    for (int c = 0; c < D; c += 32) {
+      float t[32];
+      tmem_ld32(tmem + lanes + kColO + c, t);
+      if (tid < nrows && whole) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 o = *reinterpret_cast<const float4 *>(smem + vrow * D * 4 + (((c + e) / 4) ^ (vrow & 7)) * 16);
-            t[e] = fmaf(t[e], own, o.x), t[e + 1] = fmaf(t[e + 1], own, o.y);
-            t[e + 2] = fmaf(t[e + 2], own, o.z), t[e + 3] = fmaf(t[e + 3], own, o.w);
+        for (int e = 0; e < 32; e += 8) {
+          float y[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = qi < 0 ? 0.f : t[e + k] * f;
+          if (CT != kI8 && flagged && qi >= 0) {
+            for (int k = 0; k < 8; ++k) y[k] = add_nonfinite<CT>(p, bt, b, h, qi, c + e + k, ctx, L, drafts, y[k]);
           }
+          uint4 u;
+          if (W::kQuant ? p.q_is_f16 : CT == kF16)
+            u = make_uint4(pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]), pack_f16x2(y[6], y[7]));
+          else
+            u = pack8(y);
+          *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + row + c + e) = u;
         }
-        if (vrow < nrows && whole) {
+      } else if (tid < nrows) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            float y[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = qi < 0 ? 0.f : t[e + k] * f;
-            if (CT != kI8 && flagged && qi >= 0) {
-              for (int k = 0; k < 8; ++k) y[k] = add_nonfinite<CT>(p, bt, b, h, qi, c + e + k, ctx, L, drafts, y[k]);
-            }
-            uint4 u;
-            if (W::kQuant ? p.q_is_f16 : CT == kF16)
-              u = make_uint4(pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]), pack_f16x2(y[6], y[7]));
-            else
-              u = pack8(y);
-            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + row + c + e) = u;
-          }
-        } else if (vrow < nrows) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4 *>(rec + c + e) = make_float4(t[e], t[e + 1], t[e + 2], t[e + 3]);
-        }
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<float4 *>(rec + c + e) = make_float4(t[e], t[e + 1], t[e + 2], t[e + 3]);
       }
-      if (vrow < nrows && !whole) *reinterpret_cast<float4 *>(rec + D) = make_float4(m, l, M, flagged ? 1.f : 0.f);
     }
+    if (tid < nrows && !whole) *reinterpret_cast<float4 *>(rec + D) = make_float4(m, l, M, flagged ? 1.f : 0.f);
     tc_fence_before();
-    if constexpr (REP == 2) ok = meet();  // the next segment's query rows go where the halves met
     }
     if (!ok) give_up();
   }
@@ -871,22 +814,23 @@ bool make_cache_map(CUtensorMap *map, const void *base, const CacheAttnParams &p
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Rows of a unit. 8-bit caches come here with more than 64 rows only.
-int wide_rows(const CacheAttnParams &p, int ct) { return p.rows <= 64 && ct != kE4M3 && ct != kI8 ? 64 : 128; }
+int64_t wide_units(const CacheAttnParams &p) {
+  return static_cast<int64_t>(p.batch) * p.hkv * ((p.rows + kTileRows - 1) / kTileRows);
+}
 
 // CTAs: as many as run at once, fewer where the longest possible sequences could not feed them.
 int wide_grid(const CacheAttnParams &p, int ct) {
-  const int64_t units = static_cast<int64_t>(p.batch) * p.hkv * ((p.rows + wide_rows(p, ct) - 1) / wide_rows(p, ct));
+  const int64_t units = wide_units(p), slots = (ct == kE4M3 || ct == kI8 ? 1 : 2) * sm_count();
   const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.block_size + kTileKeys - 1) / kTileKeys;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((ct == kE4M3 || ct == kI8 ? 1 : 2) * sm_count(), std::max(units, units * tiles / kMinTiles))));
+  return static_cast<int>(std::max<int64_t>(1, std::min(slots, std::max(units, units * tiles / kMinTiles))));
 }
 
-template <int CT, int D, int REP> int launch_wide(const WideParams &wp, const WideMaps &maps, cudaStream_t s) {
+template <int CT, int D> int launch_wide(const WideParams &wp, const WideMaps &maps, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};  // bit: device whose shared-memory limit is set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NVB200_ERR_CUDA;
   if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
-    if (cudaFuncSetAttribute(cache_attention_wide_kernel<CT, D, REP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(cache_attention_wide_kernel<CT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              Wide<CT, D>::kSmem) != cudaSuccess) {
       cudaGetLastError();
       return NVB200_ERR_CUDA;
@@ -894,33 +838,25 @@ template <int CT, int D, int REP> int launch_wide(const WideParams &wp, const Wi
     ready.fetch_or(uint64_t{1} << dev, std::memory_order_release);
   }
   const int grid = wide_grid(wp.a, CT);
-  if (int rc = launch_ex(cache_attention_wide_kernel<CT, D, REP>, dim3(grid), dim3(Wide<CT, D>::kThreads), Wide<CT, D>::kSmem, s, 1,
+  if (int rc = launch_ex(cache_attention_wide_kernel<CT, D>, dim3(grid), dim3(Wide<CT, D>::kThreads), Wide<CT, D>::kSmem, s, 1,
                          false, wp, maps))
     return rc;
-  return launch_cache_attention_merge(wp.a, CT, D, kTileRows / REP, grid, s);
-}
-
-template <int CT, int D> int launch_rep(const WideParams &wp, const WideMaps &maps, cudaStream_t s) {
-  if constexpr (!CacheType<CT>::kQuant) {
-    if (wide_rows(wp.a, CT) == 64) return launch_wide<CT, D, 2>(wp, maps, s);
-  }
-  return launch_wide<CT, D, 1>(wp, maps, s);
+  return launch_cache_attention_merge(wp.a, CT, D, kTileRows, grid, s);
 }
 
 }  // namespace
 
-bool wide_takes(const CacheAttnParams &p, int ct) {
+bool wide_takes(const CacheAttnParams &p) {
   // Boxes are runs of tokens of one page: 8 rows is the swizzle's period. A zero scale would make masked scores 0 * -inf.
   if (p.block_size % 8 != 0 || p.num_blocks > INT32_MAX || !aligned16(p.out) || !(std::fabs(p.scale_log2) > 1e-30f))
     return false;
   // Tiles are counted in 32 bits.
   const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.block_size + kTileKeys - 1) / kTileKeys;
-  const int64_t units = static_cast<int64_t>(p.hkv) * ((p.rows + wide_rows(p, ct) - 1) / wide_rows(p, ct)) * p.batch;
-  return units <= INT32_MAX / std::max<int64_t>(tiles, 1);
+  return wide_units(p) <= INT32_MAX / std::max<int64_t>(tiles, 1);
 }
 
 int64_t wide_workspace_bytes(const CacheAttnParams &p, int ct, int head_dim) {
-  return even_share_bytes(wide_grid(p, ct), wide_rows(p, ct), head_dim);
+  return even_share_bytes(wide_grid(p, ct), kTileRows, head_dim);
 }
 
 int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, void *workspace, cudaStream_t stream) {
@@ -933,10 +869,10 @@ int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, 
       !make_cache_map(&maps.v, p.v_cache, p, ct, head_dim, wp.box_rows))
     return NVB200_ERR_UNSUPPORTED;
   switch (ct) {
-    case kBf16: return head_dim == 64 ? launch_rep<kBf16, 64>(wp, maps, stream) : launch_rep<kBf16, 128>(wp, maps, stream);
-    case kF16: return head_dim == 64 ? launch_rep<kF16, 64>(wp, maps, stream) : launch_rep<kF16, 128>(wp, maps, stream);
-    case kE4M3: return head_dim == 64 ? launch_rep<kE4M3, 64>(wp, maps, stream) : launch_rep<kE4M3, 128>(wp, maps, stream);
-    default: return head_dim == 64 ? launch_rep<kI8, 64>(wp, maps, stream) : launch_rep<kI8, 128>(wp, maps, stream);
+    case kBf16: return head_dim == 64 ? launch_wide<kBf16, 64>(wp, maps, stream) : launch_wide<kBf16, 128>(wp, maps, stream);
+    case kF16: return head_dim == 64 ? launch_wide<kF16, 64>(wp, maps, stream) : launch_wide<kF16, 128>(wp, maps, stream);
+    case kE4M3: return head_dim == 64 ? launch_wide<kE4M3, 64>(wp, maps, stream) : launch_wide<kE4M3, 128>(wp, maps, stream);
+    default: return head_dim == 64 ? launch_wide<kI8, 64>(wp, maps, stream) : launch_wide<kI8, 128>(wp, maps, stream);
   }
 }
 

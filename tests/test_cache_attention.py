@@ -644,3 +644,38 @@ def test_two_calls_at_once(cuda, n):
     torch.cuda.synchronize()
     for i in range(2):
         assert torch.equal(got[i], want[i]) and all(torch.equal(x, want[i]) for x in eager[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cdt", [B16, H16, E4M3])
+@pytest.mark.parametrize("n", [2, 30, 80])
+@pytest.mark.parametrize("pages", [12, 300])
+def test_context_values_beside_the_drafts_reach_every_row(cuda, cdt, n, pages):
+    """An infinity (e4m3: a NaN code) of V in the context, in the same tile of keys as the first drafts, reaches every row;
+    beside one in a draft that only one row sees. In short and long block tables."""
+    import nanovllm_b200
+    qdt = H16 if cdt == H16 else B16
+    ctx, hq, hkv, d, bs = 100, 4, 2, 64, 16
+    q, kv, cache, table, m, _ = _problem(1, n, [ctx + n], hq, hkv, d, bs, qdt, cdt, cuda, seed=n)
+    wide = torch.zeros(1, pages, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    m[:] = torch.eye(n, dtype=torch.bool)
+    run = lambda causal_mask: nanovllm_b200.tree_attention(  # noqa: E731
+        q.to(cuda), cache[0], cache[1], torch.tensor([ctx + n], dtype=torch.int32, device=cuda), causal_mask, wide.to(cuda),
+        k_scale=cache[2], v_scale=cache[3])
+    masks = (m.to(cuda), None)
+    want = [run(x) for x in masks]
+    for j, col in ((ctx - 2, 3), (ctx + 1, 5)):
+        at = (int(table[0, j // bs]), j % bs)
+        if cdt == E4M3:
+            cache[1].view(torch.uint8)[at][0, col] = 0x7F
+        else:
+            cache[1][at][0, col] = float("inf")
+    hit = (lambda x: x.isnan()) if cdt == E4M3 else (lambda x: x == float("inf"))
+    for x, w, sees in zip(map(run, masks), want, ([1], range(1, n))):
+        assert bool(hit(x[0, :, :2, 3]).all())
+        assert [i for i in range(n) if bool(hit(x[0, i, :2, 5]).all())] == list(sees)
+        rest = torch.ones_like(x, dtype=torch.bool)
+        rest[0, :, :2, 3] = False
+        rest[0, list(sees), :2, 5] = False
+        assert torch.equal(x[rest], w[rest])
