@@ -103,7 +103,7 @@ template <int CT, int D, int NT, bool CLUSTER> struct Form {
   static_assert(!CLUSTER || kRecord <= kWarpRing, "a warp's record takes its ring's place");
   // Cluster form: the records that a CTA receives, splits * ceil(kRows / splits) rows.
   static constexpr int kReceived = kRing;
-  static constexpr int kRowsAt = kRing + (CLUSTER ? (kMaxSplits + G::kRows - 1) * G::kStride * 4 : kWarps * kRecord);
+  static constexpr int kRowsAt = kReceived + (CLUSTER ? (kMaxSplits + G::kRows - 1) * G::kStride * 4 : kWarps * kRecord);
   static constexpr int kSmem = kRowsAt + G::kRows * 16;  // merged m, l, M, flag per row
   static constexpr int kCtasPerSm = NT == 1 && 228 * 1024 / (kSmem + 1024) >= 3 ? 3 : 2;
   static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
@@ -757,8 +757,8 @@ template <int CT, int D, int NT> NarrowShape shape_of(const CacheAttnParams &p) 
 }
 
 // The one place that picks a kernel: f(cache type, head_dim, row tiles of 8) as integral constants. More than 16 rows are
-// blocks of 16 (a form with 32 rows a warp, its queries in shared memory, took 92 us where this takes 73: it has half the
-// warps, and the code is bound by dependent issue).
+// blocks of 16 (a form with 32 rows a warp, its queries in shared memory, took 92 us on 64 rows of 32 x 2048 keys where this took 73: it has
+// half the warps, and the code is bound by dependent issue).
 template <int I> using Int = std::integral_constant<int, I>;
 template <typename F> auto with_kernel(const CacheAttnParams &p, int ct, int d, F &&f) {
   auto rows = [&](auto CT, auto D) {
@@ -824,11 +824,11 @@ template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_s
 
 // Whether a call takes the wide kernel (128 rows a CTA on the 5th-generation tensor cores) rather than blocks of 16 rows of
 // this one. Measured on B200, head_dim 128, group 4, this kernel / the wide one, us, for ragged batches of (sequences x keys):
-//   16-bit cache, 64 rows:  32 x 2048  80 /  87, 32 x 4096 182 / 116, 8 x 16384 144 /  96
-//   16-bit cache, 128 rows: 32 x 2048 151 / 100, 32 x 4096 225 / 122, 8 x 16384 271 / 109
-//   8-bit cache,  64 rows:  32 x 2048  74 / 133, 32 x 4096 139 / 188, 8 x 16384 106 / 149
-//   8-bit cache,  128 rows: 32 x 2048 132 / 157, 32 x 4096 241 / 228, 8 x 16384 213 / 150
-//   8-bit cache,  256 rows: 4 x 2048   61 /  46, 8 x 16384 351 / 228
+//   16-bit cache, 64 rows:  32 x 2048  79 /  75, 32 x 4096 182 / 109, 8 x 16384 144 /  94
+//   16-bit cache, 128 rows: 32 x 2048 151 /  94, 32 x 4096 225 / 118, 8 x 16384 271 / 110
+//   8-bit cache,  64 rows:  32 x 2048  70 / 129, 32 x 4096 133 / 183, 8 x 16384 105 / 144
+//   8-bit cache,  128 rows: 32 x 2048 132 / 147, 32 x 4096 241 / 223, 8 x 16384 213 / 148
+//   8-bit cache,  256 rows: 4 x 2048   61 /  46, 8 x 16384 351 / 227
 // (8-bit tiles pass through shared memory twice there; long tables let its roles run undisturbed).
 bool prefers_wide(const CacheAttnParams &p, int ct) {
   const bool many_keys = static_cast<int64_t>(p.max_pages) * p.block_size > kFewKeys;

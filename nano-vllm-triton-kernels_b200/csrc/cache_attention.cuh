@@ -1,5 +1,5 @@
-// Shared by the two kernels of nvb200_cache_attention (cache_attention.cu: up to 16 query rows per KV head and CTA;
-// cache_attention_wide.cu: up to 128): parameters, cache element types and their conversion.
+// Shared by the kernels of nvb200_cache_attention (cache_attention.cu: up to 16 query rows per KV head and CTA;
+// cache_attention_wide.cu: up to 128; cache_attention_merge.cu): parameters, cache element types and their conversion.
 #pragma once
 
 #include "common.cuh"

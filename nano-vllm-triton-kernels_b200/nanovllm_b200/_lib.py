@@ -38,7 +38,22 @@ EXPORTS = ("nvb200_status_string", "nvb200_qk_norm_rope_kv", "nvb200_qk_norm_rop
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
 
 
-class QkNormRopeKvArgs(ctypes.Structure):
+_CODES = {_vp: "P", _i64: "q", _i32: "i", _f32: "f"}
+
+
+class _Packed(ctypes.Structure):
+    """A C struct that calls also take as the bytes of pack(...), its fields in order (a null pointer is 0): that costs a
+    third of what filling the structure does, which counts where a call's host time exceeds its kernel's."""
+
+    def __init_subclass__(cls):
+        cls.pack = struct.Struct("@" + "".join(_CODES[t] for _, t in cls._fields_)).pack
+
+    @classmethod
+    def from_param(cls, x):
+        return ctypes.byref(x) if isinstance(x, cls) else x
+
+
+class QkNormRopeKvArgs(_Packed):
     """nvb200_qk_norm_rope_kv_args (field order and types as in nvb200.h)."""
     _fields_ = [
         ("q_out", _vp), ("k_out", _vp), ("q", _vp), ("k", _vp), ("v", _vp),
@@ -69,21 +84,6 @@ class PagedDecodeArgs(ctypes.Structure):
         ("head_dim", _i32), ("block_size", _i32), ("max_blocks_per_seq", _i32), ("causal", _i32),
         ("num_splits", _i32), ("dtype", _i32), ("softmax_scale", _f32), ("status", _vp),
     ]
-
-
-_CODES = {_vp: "P", _i64: "q", _i32: "i", _f32: "f"}
-
-
-class _Packed(ctypes.Structure):
-    """A C struct that calls also take as the bytes of pack(...), its fields in order (a null pointer is 0): that costs a
-    third of what filling the structure does, which counts where a call's host time exceeds its kernel's."""
-
-    def __init_subclass__(cls):
-        cls.pack = struct.Struct("@" + "".join(_CODES[t] for _, t in cls._fields_)).pack
-
-    @classmethod
-    def from_param(cls, x):
-        return ctypes.byref(x) if isinstance(x, cls) else x
 
 
 class QuantCache(_Packed):
@@ -174,7 +174,7 @@ def _declare(lib):
     lib.nvb200_store_kvcache_quant.argtypes = [_vp, _i64, _vp, _i64, _vp, ctypes.c_int, _i64, ctypes.c_int, QuantCache,
                                                _vp, _vp]
     lib.nvb200_store_kvcache_quant.restype = ctypes.c_int
-    lib.nvb200_qk_norm_rope_kv_quant.argtypes = [ctypes.POINTER(QkNormRopeKvArgs), QuantCache, _vp]
+    lib.nvb200_qk_norm_rope_kv_quant.argtypes = [QkNormRopeKvArgs, QuantCache, _vp]
     lib.nvb200_qk_norm_rope_kv_quant.restype = ctypes.c_int
     lib.nvb200_load_kvcache_quant.argtypes = [_vp, _vp, QuantCache, _vp, _i64, _i32, _vp, _i32, _i64, ctypes.c_int,
                                               ctypes.c_int, _vp, _vp]

@@ -15,8 +15,6 @@ row with an infinity or NaN reads back as NaN throughout.
   device status word (nanovllm_b200.status()).
 * Within one call the slots other than -1 must differ from each other.
 """
-import ctypes
-
 import torch
 
 from nanovllm_b200 import _lib
@@ -122,14 +120,14 @@ def qk_norm_rope_kv_quant(
     _require(q.is_cuda, "q must be a CUDA tensor")
     for x in (k, v, positions, q_weight, k_weight, cos_sin_cache, k_cache, slot_mapping):
         _require(x.get_device() == idx, "all tensors must be on one device")
-    q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
-    k_out = torch.empty(T, Hkv, D, dtype=q.dtype, device=dev) if write_k else None
+    q_out = q.new_empty((T, Hq, D))
+    k_out = q.new_empty((T, Hkv, D)) if write_k else None
     if T == 0:
         return q_out, k_out
-    a = _lib.QkNormRopeKvArgs(
-        q_out.data_ptr(), _lib.ptr(k_out), q.data_ptr(), k.data_ptr(), v.data_ptr(), sq[0], sk[0], sv[0],
+    a = _lib.QkNormRopeKvArgs.pack(
+        q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), sq[0], sk[0], sv[0],
         positions.data_ptr(), slot_mapping.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
-        cos_sin_cache.data_ptr(), cos_sin_cache.stride(0), cos_sin_cache.shape[0], None, None, 0, T, Hq, Hkv, D, eps,
+        cos_sin_cache.data_ptr(), cos_sin_cache.stride(0), cos_sin_cache.shape[0], 0, 0, 0, T, Hq, Hkv, D, eps,
         _lib.status_word(dev).data_ptr())
     cache = _cache_arg(k_cache, v_cache, k_scale, v_scale, shape)
     with _lib.device_of(dev):
