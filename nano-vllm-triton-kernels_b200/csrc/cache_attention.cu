@@ -92,7 +92,8 @@ template <int CT, int D, int NT> struct Geometry {
 // What the two forms of the kernel lay out differently. The warps' records of their partial results lie, in the cluster
 // form, where a CTA has one segment, in the warps' own rings; in the even-share form, where the next segment's tiles are
 // landing there already, beside them. The saving lets three CTAs of the cluster form share an SM for at most 8 rows (256
-// sequences of 300 keys, e4m3: 60 -> 49 us; six warps a CTA in the same memory: 56 us).
+// sequences of 300 keys, e4m3: 60 -> 49 us; six warps a CTA in the same memory: 56 us). At head_dim 64 both forms fit three
+// times with 16 rows too (32 x 16 drafts, group 4, 2048 keys, bf16: 57 -> 48 us); at 128 their registers do not.
 template <int CT, int D, int NT, bool CLUSTER> struct Form {
   using G = Geometry<CT, D, NT>;
   static constexpr int kWarpRing = G::kStages * G::kStageBytes;
@@ -105,7 +106,7 @@ template <int CT, int D, int NT, bool CLUSTER> struct Form {
   static constexpr int kReceived = kRing;
   static constexpr int kRowsAt = kReceived + (CLUSTER ? (kMaxSplits + G::kRows - 1) * G::kStride * 4 : kWarps * kRecord);
   static constexpr int kSmem = kRowsAt + G::kRows * 16;  // merged m, l, M, flag per row
-  static constexpr int kCtasPerSm = NT == 1 && 228 * 1024 / (kSmem + 1024) >= 3 ? 3 : 2;
+  static constexpr int kCtasPerSm = (NT == 1 || D == 64) && 228 * 1024 / (kSmem + 1024) >= 3 ? 3 : 2;
   static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
