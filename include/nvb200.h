@@ -395,7 +395,8 @@ NVB200_API int nvb200_load_kvcache_quant(void *key, void *value, const nvb200_qu
  * whatever its bits. Where seqlens[b] < m, the first m - seqlens[b] new tokens are not in the cache and seen by no row.
  *   q: [batch, n, num_q_heads, head_dim] with the given strides, unit last stride; dtype bf16 or fp16.
  *   cache_dtype: = dtype (16-bit cache, strides as given, unit last stride), or NVB200_E4M3 / NVB200_I8 with k_scale and
- *     v_scale contiguous [num_blocks, num_kv_heads, block_size] (see nvb200_quant_cache).
+ *     v_scale contiguous [num_blocks, num_kv_heads, block_size] (see nvb200_quant_cache), at any 4-byte aligned address
+ *     (16-byte aligned ones can take the kernel for many query rows).
  *   num_splits: 0: chosen from the sizes (even shares of all sequences' keys over the GPU, or a cluster of CTAs per
  *     sequence); 1..8: that many CTAs (a thread-block cluster) share each sequence's keys.
  *   block_table, seqlens, softmax_scale, status: as for nvb200_paged_decode_attention. Keys whose block-table

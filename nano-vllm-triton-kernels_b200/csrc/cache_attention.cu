@@ -869,7 +869,7 @@ int prepare_attention(const nvb200_cache_attention_args *a, CacheAttnParams &p, 
   p.q_head_stride = a->q_head_stride;
   p.k_cache = static_cast<const uint8_t *>(a->k_cache), p.v_cache = static_cast<const uint8_t *>(a->v_cache);
   p.blk_stride = a->cache_block_stride, p.tok_stride = a->cache_token_stride, p.head_stride = a->cache_head_stride;
-  p.num_blocks = a->num_blocks, p.k_scale = a->k_scale, p.v_scale = a->v_scale;
+  p.num_blocks = a->num_blocks, p.k_scale = quant ? a->k_scale : nullptr, p.v_scale = quant ? a->v_scale : nullptr;
   p.block_table = a->block_table, p.bt_stride = a->block_table_stride;
   p.max_pages = a->block_table ? a->max_blocks_per_seq : 1;
   p.seqlens = a->seqlens, p.draft_lens = a->draft_lens;

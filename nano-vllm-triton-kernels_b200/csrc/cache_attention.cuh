@@ -294,7 +294,7 @@ __device__ __noinline__ float add_nonfinite(const CacheAttnParams &p, const int3
 }  // namespace
 
 // The wide kernel (cache_attention_wide.cu). NVB200_ERR_UNSUPPORTED where it does not take the call (pages whose size is
-// not a multiple of 8 tokens, cache strides that no tensor map describes).
+// not a multiple of 8 tokens, row scales off a 16-byte boundary, cache strides that no tensor map describes).
 bool wide_takes(const CacheAttnParams &p);
 int64_t wide_workspace_bytes(const CacheAttnParams &p, int ct, int head_dim);
 int launch_cache_attention_wide(const CacheAttnParams &p, int ct, int head_dim, void *workspace, cudaStream_t stream);

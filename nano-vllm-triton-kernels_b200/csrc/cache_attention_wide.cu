@@ -850,6 +850,8 @@ bool wide_takes(const CacheAttnParams &p) {
   // Boxes are runs of tokens of one page: 8 rows is the swizzle's period. A zero scale would make masked scores 0 * -inf.
   if (p.block_size % 8 != 0 || p.num_blocks > INT32_MAX || !aligned16(p.out) || !(std::fabs(p.scale_log2) > 1e-30f))
     return false;
+  // Row scales (NULL for 16-bit caches) come by bulk copies: whole runs of 8 tokens, so their bases decide the alignment.
+  if (!aligned16(p.k_scale) || !aligned16(p.v_scale)) return false;
   // Tiles are counted in 32 bits.
   const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.block_size + kTileKeys - 1) / kTileKeys;
   return wide_units(p) <= INT32_MAX / std::max<int64_t>(tiles, 1);

@@ -679,3 +679,69 @@ def test_context_values_beside_the_drafts_reach_every_row(cuda, cdt, n, pages):
         rest[0, :, :2, 3] = False
         rest[0, list(sees), :2, 5] = False
         assert torch.equal(x[rest], w[rest])
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Row scales at any address.
+
+def _host_args(**kw):
+    """nvb200_cache_attention_args of 2 x 4 tokens, 8 query heads over one KV head, for host-side queries (nothing runs)."""
+    from nanovllm_b200 import _lib
+    a = _lib.CacheAttentionArgs()
+    for p in ("out", "q", "k_cache", "v_cache", "block_table", "seqlens", "k_scale", "v_scale"):
+        setattr(a, p, 1 << 20)
+    a.num_blocks, a.batch, a.queries_per_seq, a.num_q_heads, a.num_kv_heads, a.head_dim = 64, 2, 4, 8, 1, 128
+    a.q_batch_stride, a.q_token_stride, a.q_head_stride = 4096, 1024, 128
+    a.cache_block_stride, a.cache_token_stride, a.cache_head_stride = 64 * 128, 128, 128
+    a.block_size, a.max_blocks_per_seq, a.dtype, a.cache_dtype, a.softmax_scale = 64, 16, _lib.BF16, _lib.E4M3, 0.1
+    a.causal = 1
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("field", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("offset", [4, 8, 12])
+def test_scales_off_a_16_byte_boundary_do_not_take_the_wide_kernel(field, offset):
+    """The wide kernel brings row scales by bulk copies, whose sources are 16-byte aligned. In a short block table it is the
+    only form that needs a workspace, so the size tells which kernel a call takes."""
+    from nanovllm_b200 import _lib
+    size = _lib.lib().nvb200_cache_attention_workspace_size
+    many = dict(queries_per_seq=40)  # 320 rows
+    assert size(_host_args(**many)) > 0
+    assert size(_host_args(**many, **{field: (1 << 20) + offset})) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cdt", [E4M3, I8])
+@pytest.mark.parametrize("n,width", [(1, 0), (3, 0), (40, 0), (40, 80), (80, 0)])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_scales_at_any_address(cuda, cdt, n, width, offset):
+    """Scales carved out of a larger buffer: written, read back and attended as at the buffer's start."""
+    import nanovllm_b200
+    lens, hq, hkv, d, bs = [n + 130, n + 7], 4, 1, 128, 64
+    q, kv, cache, table, m, drafts = _problem(2, n, lens, hq, hkv, d, bs, B16, cdt, cuda, seed=n)
+    table = torch.cat([table, table.new_zeros(2, max(0, width - table.shape[1]))], 1)
+    for i in (2, 3):
+        pool = torch.full((cache[i].numel() + 8,), -1.0, device=cuda)
+        view = pool[offset:offset + cache[i].numel()].view(cache[i].shape)
+        view.copy_(cache[i])
+        cache[i] = view
+        assert view.data_ptr() % 16 == 4 * offset
+    nanovllm_b200.status(cuda, clear=True)
+    got = nanovllm_b200.tree_attention(q.to(cuda), cache[0], cache[1], torch.tensor(lens, dtype=torch.int32, device=cuda),
+                                       m.to(cuda), table.to(cuda), k_scale=cache[2], v_scale=cache[3])
+    _check(got, q, kv, table, lens, m, drafts, d ** -0.5, cdt)
+    cu = torch.tensor([0, lens[0], sum(lens)], dtype=torch.int32, device=cuda)
+    back = nanovllm_b200.load_kvcache_quant(*cache, table.to(cuda), cu, sum(lens), dtype=torch.float32)
+    for x, values in zip(back, kv):
+        want = torch.cat([values[table[b].long()].flatten(0, 1)[:lens[b]] for b in range(2)])
+        assert torch.equal(x.cpu(), want.float())
+    slot = int(table[0, 0]) * bs
+    nanovllm_b200.store_kvcache_quant(back[0][5:6], back[1][5:6], *cache, torch.tensor([slot], device=cuda))
+    again = nanovllm_b200.load_kvcache_quant(*cache, table.to(cuda), cu, sum(lens), dtype=torch.float32)
+    # Values that came from a row of the cache: quantised again by the definition.
+    for x, y in zip(back, again):
+        codes, scale = cm.quantise_rows(x[5:6].cpu(), cdt)
+        assert torch.equal(y[0].cpu(), codes.float()[0] * scale[0][:, None]) and torch.equal(x[1:], y[1:])
+    assert nanovllm_b200.status(cuda) == 0
