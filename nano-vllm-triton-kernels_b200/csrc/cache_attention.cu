@@ -512,8 +512,8 @@ __global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm
   };
 
   int stage = 0;  // of the tile to fold next
-  bool dirty = false;  // an infinity or NaN was taken out of a V tile
   do {
+    bool dirty = false;  // an infinity or NaN was taken out of a V tile of this segment
     const int b = seg.b, h = seg.unit / seg.s.blocks, row0 = (seg.unit - h * seg.s.blocks) * G::kRows;
     const int L = seg.s.L, drafts = seg.s.drafts, ctx = L - drafts;  // ctx < 0: the first new tokens are not in the cache
     const int open = masked ? max(ctx, 0) : L;  // every row sees the keys below this
@@ -653,9 +653,11 @@ __global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm
       // l > 0 wherever a key was seen; NaN (a NaN score) is passed on.
       const float f = x.y == 0.f ? 0.f : (C::kQuant ? exp2f(x.z - x.x) : 1.f) / x.y;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        y[k] = qi < drafts && x.y != 0.f ? y[k] * f : 0.f;
-        if (CT != kI8 && x.w != 0.f && qi < drafts) y[k] = add_nonfinite<CT>(p, bt, b, h, qi, d + k, ctx, L, drafts, y[k]);
+      for (int k = 0; k < 4; ++k) y[k] = qi < drafts && x.y != 0.f ? y[k] * f : 0.f;
+      if (CT != kI8 && x.w != 0.f && qi < drafts) {
+        const Columns<4> more = nonfinite_sum<CT, 4>(p, bt, b, h, qi, d, ctx, drafts);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] += more.v[k];
       }
       const bool f16 = C::kQuant ? p.q_is_f16 : CT == kF16;
       const uint32_t lo = f16 ? pack_f16x2(y[0], y[1]) : pack_bf16x2(y[0], y[1]);

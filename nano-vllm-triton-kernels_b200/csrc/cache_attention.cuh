@@ -267,25 +267,63 @@ NVB200_DEVICE int page_of(const CacheAttnParams &p, int j) {
 }
 
 // Infinities and NaN of V among the new tokens are taken out of the tiles (0 * inf is NaN in a matrix instruction, and a
-// row may not see them); a row that does see one gets it here, where it decides column d whatever its weight. y: the
-// row's output without them.
-template <int CT>
-__device__ __noinline__ float add_nonfinite(const CacheAttnParams &p, const int32_t *bt, int b, int h, int qi, int d, int ctx, int L,
-                                  int drafts, float y) {
-  for (int k = 0; k < drafts; ++k) {
-    const int j = ctx + k;
-    if (j < 0 || j >= L || !(p.mask ? p.mask[b * p.mask_batch_stride + qi * p.mask_row_stride + k] != 0 : k <= qi))
-      continue;
-    const int page = page_of(p, j);
-    const int64_t blk = bt ? __ldg(bt + page) : b;
-    if (blk < 0 || blk >= p.num_blocks) continue;
-    const int64_t at = blk * p.blk_stride + (j - page * p.block_size) * p.tok_stride + h * p.head_stride + d;
-    if constexpr (CacheType<CT>::kQuant) {
-      if ((__ldg(p.v_cache + at) & 0x7Fu) == 0x7Fu) y = __uint_as_float(0x7FC00000u);
-    } else {
-      const uint16_t u = __ldg(reinterpret_cast<const uint16_t *>(p.v_cache) + at);
-      if (nonfinite_bits<CT>(u))
-        y += CT == kBf16 ? __uint_as_float(static_cast<uint32_t>(u) << 16) : __half2float(__ushort_as_half(u));
+// row may not see them); a row that does see one gets it from here, where it decides a column whatever its weight: what those
+// that token qi sees add to columns d .. d + N - 1 of KV head h (d a multiple of N: one piece of the row). Only for segments
+// that held one. The loads of eight keys are in flight together, so the scan of the largest call (4096 new tokens, 16 pieces
+// of a row) takes some milliseconds where a key at a time took a good part of the second that waiting warps allow.
+template <int N> struct Columns {
+  float v[N];
+};
+template <int CT, int N>
+__device__ __noinline__ Columns<N> nonfinite_sum(const CacheAttnParams &p, const int32_t *bt, int b, int h, int qi, int d,
+                                                 int ctx, int drafts) {
+  constexpr int kBatch = 8, kWords = N * CacheType<CT>::kBytes / 4;
+  Columns<N> y{};
+  const uint8_t *mask = p.mask ? p.mask + b * p.mask_batch_stride + qi * p.mask_row_stride : nullptr;
+  for (int k0 = 0; k0 < drafts; k0 += kBatch) {
+    int blk[kBatch];
+    uint32_t w[kBatch][kWords];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int k = k0 + i;
+      const bool seen = k < drafts && ctx + k >= 0 && (mask ? __ldg(mask + k) != 0 : k <= qi);
+      blk[i] = !seen ? -1 : (bt ? __ldg(bt + page_of(p, ctx + k)) : b);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) w[i][e] = 0u;
+      if (blk[i] >= 0 && blk[i] < p.num_blocks) {
+        const int j = ctx + k0 + i;
+        const int64_t at = blk[i] * p.blk_stride + (j - page_of(p, j) * p.block_size) * p.tok_stride + h * p.head_stride + d;
+        const uint8_t *from = p.v_cache + at * CacheType<CT>::kBytes;
+        if constexpr (kWords == 4) {
+          const uint4 u = __ldg(reinterpret_cast<const uint4 *>(from));
+          w[i][0] = u.x, w[i][1] = u.y, w[i][2] = u.z, w[i][3] = u.w;
+        } else if constexpr (kWords == 2) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2 *>(from));
+          w[i][0] = u.x, w[i][1] = u.y;
+        } else {
+          w[i][0] = __ldg(reinterpret_cast<const uint32_t *>(from));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      uint32_t found = 0;
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) found |= nonfinite_bits<CT>(w[i][e]);
+      if (found == 0) continue;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if constexpr (CacheType<CT>::kQuant) {
+          if ((w[i][e / 4] >> (8 * (e % 4)) & 0x7Fu) == 0x7Fu) y.v[e] = __uint_as_float(0x7FC00000u);
+        } else {
+          const uint32_t u = w[i][e / 2] >> (16 * (e % 2)) & 0xFFFFu;
+          if (nonfinite_bits<CT>(u))
+            y.v[e] += CT == kBf16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(u)));
+        }
+      }
     }
   }
   return y;

@@ -58,13 +58,14 @@ __global__ void __launch_bounds__(kMergeThreads)
   }
   const int row_all = row0 + r, qi = row_all / p.group, gq = row_all - qi * p.group;
   const float f = l == 0.f ? 0.f : (C::kQuant ? exp2f(M - m) : 1.f) / l;
+  Columns<4> more{};
+  if (CT != kI8 && flag != 0.f && qi < x.drafts)
+    more = nonfinite_sum<CT, 4>(p, p.block_table ? p.block_table + x.b * p.bt_stride : nullptr, x.b, h, qi, d, x.L - x.drafts,
+                                x.drafts);
   uint16_t out[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    float v = qi < x.drafts ? y[k] * f : 0.f;
-    if (CT != kI8 && flag != 0.f && qi < x.drafts)
-      v = add_nonfinite<CT>(p, p.block_table ? p.block_table + x.b * p.bt_stride : nullptr, x.b, h, qi, d + k, x.L - x.drafts,
-                            x.L, x.drafts, v);
+    const float v = (qi < x.drafts ? y[k] * f : 0.f) + more.v[k];
     out[k] = (C::kQuant ? p.q_is_f16 : CT == kF16) ? __half_as_ushort(__float2half_rn(v))
                                                    : __bfloat16_as_ushort(__float2bfloat16_rn(v));
   }

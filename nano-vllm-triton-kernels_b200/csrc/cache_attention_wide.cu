@@ -159,7 +159,11 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
   const uint32_t b_rfull = hdr + 200, b_rempty = hdr + 264;              // up to 8 each
   const uint32_t live_slot = hdr + 328, raw_live = hdr + 392;            // 64-bit words: up to 8 each
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + W::kOffHdr + 456);
-  const uint32_t failed = hdr + 460, dirty = hdr + 464;  // flags
+  const uint32_t failed = hdr + 460;  // flag
+  // Word q % 4 holds q + 1 once segment q of the CTA's had an infinity or NaN taken out of V. V of a tile is converted once
+  // the P V two tiles before it is done, so at most two segments ahead of the one that the softmax finishes.
+  const uint32_t dirty = hdr + 464;
+  auto dirty_word = [&](int q) { return dirty + 4 * (q & 3); };
 
   if (tid == 0) {
     for (int i = 0; i < W::NK; ++i) mbar_init(b_kfull + 8 * i, W::kQuant ? W::kConvWarps : 1), mbar_init(b_kempty + 8 * i, 1);
@@ -167,7 +171,8 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
     for (int i = 0; i < 2; ++i) mbar_init(b_sfull + 8 * i, 2), mbar_init(b_pready + 8 * i, 4), mbar_init(b_pv + 8 * i, 1);
     mbar_init(b_q, 4);
     for (int i = 0; i < W::NR; ++i) mbar_init(b_rfull + 8 * i, 1), mbar_init(b_rempty + 8 * i, W::kConvWarps);
-    st_shared_u32(failed, 0u), st_shared_u32(dirty, 0u);
+    st_shared_u32(failed, 0u);
+    for (int i = 0; i < 4; ++i) st_shared_u32(dirty + 4 * i, 0u);
     fence_mbar_init();
   }
   if (warp == 5) tmem_alloc(smem_addr(tmem_slot), kTmemCols);
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
 
   const bool masked = p.mask != nullptr || p.causal;
   // Of the current segment: first tile's first key, end of its keys; keys before the new tokens; every row sees the keys
-  // below `open`; whether a row may not see a key that others see (V must then be finite: see add_nonfinite).
+  // below `open`; whether a row may not see a key that others see (V must then be finite: see nonfinite_sum).
   auto first_key = [&]() { return seg.t0 * kTileKeys; };
   auto end_key = [&]() { return min(static_cast<int64_t>(seg.s.L), static_cast<int64_t>(seg.t0 + seg.n) * kTileKeys); };
   auto context = [&]() { return seg.s.L - seg.s.drafts; };
@@ -379,8 +384,8 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
       constexpr int kRowsPer = 128 / kChunks;    // rows that the 128 threads cover at a time
       const int r8 = (ct & 7) | (ct >> 3) / kChunks * 8, ch = (ct >> 3) % kChunks;
       // Converts a raw tile to an operand tile; rows whose bit of `live` is clear become zeros, and from row `finite` on
-      // e4m3's NaN codes too.
-      auto convert = [&](int src, int dst, unsigned long long live, int finite) {
+      // e4m3's NaN codes too (q: the segment).
+      auto convert = [&](int src, int dst, unsigned long long live, int finite, int q) {
         uint4 u[kTileKeys / kRowsPer];  // all loads before the first store
 #pragma unroll
         for (int k = 0; k < kTileKeys / kRowsPer; ++k) {
@@ -400,7 +405,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
               const uint32_t bad = nonfinite_bits<CT>(w[e]);
               w[e] &= ~bad, found |= bad;
             }
-            if (found) st_shared_u32(dirty, 1u);
+            if (found) st_shared_u32(dirty_word(q), q + 1);
           }
           uint4 x, y;
           codes_to_f16<CT>(w[0], x.x, x.y), codes_to_f16<CT>(w[1], x.z, x.w);
@@ -418,7 +423,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
         const int st = i % W::NR, slot = i % W::kSlots, sk = i % W::NK;
         if (!wait(b_rfull + 8 * st, (i / W::NR) & 1) || !wait(b_kempty + 8 * sk, ((i / W::NK) & 1) ^ 1)) return false;
         const unsigned long long live = live_of(st);
-        convert(W::kOffRaw + st * 2 * W::kRawBytes, W::kOffK + sk * W::kOpBytes, live, kTileKeys);
+        convert(W::kOffRaw + st * 2 * W::kRawBytes, W::kOffK + sk * W::kOpBytes, live, kTileKeys, 0);
         if (ct < kTileKeys) {
           // The key's scales; zeros where it is none (its slot of the raw tile was not loaded).
           const bool is = (live >> ct) & 1ull;
@@ -446,7 +451,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
       bool ok = convert_k(0);
       const int total = u1 - u0;
       int i = 0;
-      for (; seg.n > 0 && ok; next()) {
+      for (int q = 0; seg.n > 0 && ok; next(), ++q) {
         const bool hides = hides_keys();
         for (int t = 0; t < seg.n; ++t, ++i) {
           if (i + 1 < total) ok = convert_k(i + 1);
@@ -454,7 +459,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
           ok = ok && wait(b_vempty + 8 * sv, ((i / W::NV) & 1) ^ 1);
           if (!ok) break;
           convert(W::kOffRaw + st * 2 * W::kRawBytes + W::kRawBytes, W::kOffV + sv * W::kOpBytes, live_of(st),
-                  hides ? open_below() - (first_key() + t * kTileKeys) : kTileKeys);
+                  hides ? open_below() - (first_key() + t * kTileKeys) : kTileKeys, q);
           arrive(b_vfull + 8 * sv);
           arrive(b_rempty + 8 * st);
         }
@@ -465,9 +470,9 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
     // ---------------------------------------------------------------- softmax: thread = row
     bool ok = true;
     int i = 0;  // tile of the CTA
-    for (; seg.n > 0 && ok; next()) {
+    for (int q = 0; seg.n > 0 && ok; next(), ++q) {
     const int b = seg.b, h = seg.unit / seg.s.blocks, row0 = (seg.unit - h * seg.s.blocks) * kTileRows;
-    const int nrows = min(kTileRows, p.rows - row0), L = seg.s.L, drafts = seg.s.drafts, ctx = context();
+    const int nrows = min(kTileRows, p.rows - row0), drafts = seg.s.drafts, ctx = context();
     const int js = first_key(), je = static_cast<int>(end_key()), open = open_below();
     const bool hides = hides_keys();
     const int32_t *bt = table_of();
@@ -593,7 +598,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
                 const uint32_t bad = nonfinite_bits<CT>(w[e]);
                 w[e] &= ~bad, change |= bad;
               }
-              if (change) st_shared_u32(dirty, 1u);
+              if (change) st_shared_u32(dirty_word(q), q + 1);
             }
             if (change) st_shared_v4(at, u);
           }
@@ -748,7 +753,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
 
     if constexpr (!W::kQuant) M = m;
     const bool whole = seg.n == seg.s.tiles;
-    const bool flagged = ld_shared_u32(dirty) != 0u;
+    const bool flagged = ld_shared_u32(dirty_word(q)) == static_cast<uint32_t>(q + 1);
     const int gq = r - qi_raw * p.group;
     const float f = l == 0.f ? 0.f : (W::kQuant ? exp2f(M - m) : 1.f) / l;
     float *rec = p.records + (static_cast<int64_t>(record_slot(blockIdx.x, seg.unit_u, T, G)) * kTileRows + tid) * (D + 4);
@@ -764,7 +769,9 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
 #pragma unroll
           for (int k = 0; k < 8; ++k) y[k] = qi < 0 ? 0.f : t[e + k] * f;
           if (CT != kI8 && flagged && qi >= 0) {
-            for (int k = 0; k < 8; ++k) y[k] = add_nonfinite<CT>(p, bt, b, h, qi, c + e + k, ctx, L, drafts, y[k]);
+            const Columns<8> more = nonfinite_sum<CT, 8>(p, bt, b, h, qi, c + e, ctx, drafts);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] += more.v[k];
           }
           uint4 u;
           if (W::kQuant ? p.q_is_f16 : CT == kF16)

@@ -745,3 +745,123 @@ def test_scales_at_any_address(cuda, cdt, n, width, offset):
         codes, scale = cm.quantise_rows(x[5:6].cpu(), cdt)
         assert torch.equal(y[0].cpu(), codes.float()[0] * scale[0][:, None]) and torch.equal(x[1:], y[1:])
     assert nanovllm_b200.status(cuda) == 0
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Infinities and NaN of V among the drafts, in large trees and beside other sequences.
+
+def _same_nonfinite(got, ref):
+    """got has ref's infinities and NaN where ref has any; the finite places are left to _check's tolerance."""
+    got, bad = got.double().cpu(), ~torch.isfinite(ref)
+    assert torch.equal(torch.nan_to_num(got[bad], nan=7.0, posinf=1.0, neginf=-1.0),
+                       torch.nan_to_num(ref[bad], nan=7.0, posinf=1.0, neginf=-1.0))
+    return bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cdt", [B16, H16, E4M3])
+@pytest.mark.parametrize("n,group,pages", [(5, 2, 20), (20, 2, 200), (30, 4, 20), (160, 1, 20), (90, 3, 200)])
+@pytest.mark.parametrize("mask", ["tree", "chain"])
+def test_infinities_of_several_drafts(cuda, cdt, n, group, pages, mask):
+    """Several drafts with infinities of both signs and NaN in some columns, in both kernels and their merges: each row has the
+    sum of those it sees."""
+    import nanovllm_b200
+    hkv, d, bs, lens = 2, 64, 16, [n + 75, n + 3]
+    qdt = H16 if cdt == H16 else B16
+    q, kv, cache, table, m, drafts = _problem(2, n, lens, group * hkv, hkv, d, bs, qdt, cdt, cuda, seed=n, mask=mask)
+    wide = torch.zeros(2, pages, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    g = torch.Generator().manual_seed(3)
+    values = kv[1].double().clone()
+    for b in range(2):
+        for k in [0, n - 1] + torch.randint(0, n, (6,), generator=g).tolist():
+            j = lens[b] - n + k
+            at = (int(table[b, j // bs]), j % bs, int(torch.randint(0, hkv, (1,), generator=g)))
+            for col in torch.randint(0, d, (5,), generator=g).tolist():
+                x = [float("inf"), -float("inf"), float("nan")][int(torch.randint(0, 3, (1,), generator=g))]
+                if cdt == E4M3:
+                    x = float("nan")
+                    cache[1].view(torch.uint8)[at][col] = 0x7F if col % 2 else 0xFF
+                else:
+                    cache[1][at][col] = x
+                values[at][col] = x
+    nanovllm_b200.status(cuda, clear=True)
+    got = nanovllm_b200.tree_attention(q.to(cuda), cache[0], cache[1], torch.tensor(lens, dtype=torch.int32, device=cuda),
+                                       None if m is None else m.to(cuda), wide.to(cuda), k_scale=cache[2], v_scale=cache[3])
+    assert nanovllm_b200.status(cuda) == 0
+    # Column by column with and without the values that are not finite: a sum over the seen drafts' ones.
+    ref, spread, reach = cm.cache_attention(q, kv[0], values, lens, table, m, drafts, d ** -0.5)
+    bad = _same_nonfinite(got, ref)
+    assert bool(bad.any()) and not bool(bad.all())
+    clean = torch.nan_to_num(values, nan=0.0, posinf=0.0, neginf=0.0)
+    ref, spread, reach = cm.cache_attention(q, kv[0], clean, lens, table, m, drafts, d ** -0.5)
+    tol = _tolerance(ref, spread, reach, qdt, cdt, max(lens), float(clean.abs().max()), d)
+    assert bool(((got.double().cpu() - ref).abs() <= tol)[~bad].all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cdt", [B16, E4M3])
+@pytest.mark.parametrize("n,pages", [(3, 8), (24, 8), (40, 130), (140, 8)])
+def test_one_sequence_with_infinities_among_many(cuda, cdt, n, pages):
+    """More units than the GPU holds, so that a CTA has several, and one sequence whose drafts hold infinities or NaN: the
+    other sequences' results keep their bits, and its own are the definition's."""
+    import nanovllm_b200
+    B, hq, hkv, d, bs = 260, 4, 2, 64, 32
+    g = torch.Generator().manual_seed(n)
+    lens = [n + int(x) for x in torch.randint(0, 60, (B,), generator=g)]
+    q, kv, cache, table, m, drafts = _problem(B, n, lens, hq, hkv, d, bs, B16, cdt, cuda, seed=n)
+    wide = torch.zeros(B, pages, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    args = (q.to(cuda), cache[0], cache[1], torch.tensor(lens, dtype=torch.int32, device=cuda), m.to(cuda), wide.to(cuda))
+    run = lambda: nanovllm_b200.tree_attention(*args, k_scale=cache[2], v_scale=cache[3])  # noqa: E731
+    want = run()
+    sick = 101
+    values = kv[1].double().clone()
+    for k in range(0, n, 2):
+        j = lens[sick] - n + k
+        at = (int(table[sick, j // bs]), j % bs)
+        if cdt == E4M3:
+            cache[1].view(torch.uint8)[at][:, 9] = 0x7F
+        else:
+            cache[1][at][:, 9] = float("inf")
+        values[at][:, 9] = float("nan") if cdt == E4M3 else float("inf")
+    nanovllm_b200.status(cuda, clear=True)
+    got = run()
+    assert nanovllm_b200.status(cuda) == 0
+    well = [b for b in range(B) if b != sick]
+    assert torch.equal(got[well], want[well])
+    one = [x[sick:sick + 1] for x in (q, table, m)]
+    ref, _, _ = cm.cache_attention(one[0], kv[0], values, lens[sick:sick + 1], one[1], one[2], [n], d ** -0.5)
+    bad = _same_nonfinite(got[sick:sick + 1], ref)
+    assert bool(bad.any()) and torch.equal(got[sick:sick + 1].cpu()[~bad], want[sick:sick + 1].cpu()[~bad])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cdt", [B16, E4M3])
+@pytest.mark.parametrize("bs", [12, 64])
+def test_the_largest_tree_with_every_value_infinite(cuda, cdt, bs):
+    """4096 drafts whose values are all infinite (e4m3: NaN): what rows pick up from them ends well inside the waits' limit, in
+    the warp-level kernel (pages of 12 tokens) and the wide one."""
+    import nanovllm_b200
+    n, d, ctx = 4096, 128, 100
+    pages = -(-(ctx + n) // bs)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda)[None]
+    cache = [torch.zeros(pages, bs, 1, d, dtype=torch.uint8 if cdt == E4M3 else cdt, device=cuda) for _ in range(2)]
+    flat = cache[1].view(-1, d)
+    flat[ctx:ctx + n] = 0x7F if cdt == E4M3 else float("inf")
+    kw = {}
+    if cdt == E4M3:
+        cache = [c.view(E4M3) for c in cache]
+        kw = dict(k_scale=torch.ones(pages, 1, bs, device=cuda), v_scale=torch.ones(pages, 1, bs, device=cuda))
+    q = torch.ones(1, n, 1, d, dtype=B16, device=cuda)
+    nanovllm_b200.status(cuda, clear=True)
+    lens = torch.tensor([ctx + n], dtype=torch.int32, device=cuda)
+    got = nanovllm_b200.tree_attention(q, *cache, lens, None, table, **kw)
+    assert nanovllm_b200.status(cuda) == 0
+    assert bool(got.isnan().all()) if cdt == E4M3 else bool((got == float("inf")).all())
+    none = torch.zeros(n, n, dtype=torch.bool, device=cuda)
+    none[7, 4000] = True
+    got = nanovllm_b200.tree_attention(q, *cache, lens, none, table, **kw)
+    assert nanovllm_b200.status(cuda) == 0
+    hit = got.isnan() if cdt == E4M3 else got == float("inf")
+    assert bool(hit[0, 7].all()) and int(hit.sum()) == d and not bool(got[~hit].any())
