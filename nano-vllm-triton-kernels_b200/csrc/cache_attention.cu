@@ -12,7 +12,10 @@
 // 8-bit caches run on fp16 matrix instructions: e4m3 and int8 codes are exact in fp16 (one conversion per two codes), and
 // the query row is brought to fp16 by an exact power of two, so the only roundings are those of p and the output.
 // The weights p_j vs_j carry the row scales, whose range fp16 does not have; they are held relative to M, the running
-// maximum of s_j log2 e + (binary exponent of vs_j) + 1, which keeps each in [0, 1] with the largest near 1.
+// maximum of s_j log2 e + (binary exponent of vs_j) + 1. fp16 weights (8-bit and fp16 caches) are held 2^kWeightUp times as
+// large, the largest in (2^13, 2^14]: fp16's smallest step, 2^-24, is then 2^-37 of it or less, where weights of at most 1
+// would vanish below 2^-25, and with them what thousands of keys beside one that takes almost the whole softmax add up to.
+// The sums l carry the same factor. bf16 weights have fp32's range and stay at most 1.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -25,6 +28,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr float kWeightUp = 14.f;
 constexpr int kMinTiles = 16;  // of a CTA in the even-share form, where there are too few for all
 
 NVB200_DEVICE void cp_async16(uint32_t dst, const void *src, uint32_t src_bytes) {
@@ -247,7 +251,7 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<
   uint32_t pb[KB][NT][2];  // weights as the second operand of V^T P^T
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    float mu[2], cw[2], ao[2];
+    float up[2], cw[2], ao[2];  // up: what turns a score into its weight's exponent
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float mt = st.m[n][e], Mt = st.M[n][e];
@@ -261,13 +265,14 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
         if constexpr (C::kQuant) Mt = fmaxf(Mt, __shfl_xor_sync(0xffffffffu, Mt, o));
       }
-      mu[e] = mt == -INFINITY ? 0.f : mt;  // no key seen yet: any finite reference
-      const float al = ex2_approx_ftz(st.m[n][e] - mu[e]);
+      const float mu = mt == -INFINITY ? 0.f : mt;  // no key seen yet: any finite reference
+      up[e] = (C::kBf16Mma ? 0.f : kWeightUp) - mu;
+      const float al = ex2_approx_ftz(st.m[n][e] - mu);
       ao[e] = al, cw[e] = 1.f;
       if constexpr (C::kQuant) {
         const float Mu = Mt == -INFINITY ? 0.f : Mt;
         ao[e] = ex2_approx_ftz(st.M[n][e] - Mu);
-        cw[e] = ex2_approx_ftz(mu[e] - Mu);
+        cw[e] = ex2_approx_ftz(mu - Mu);
         st.M[n][e] = Mt;
       }
       st.m[n][e] = mt;
@@ -280,7 +285,7 @@ NVB200_DEVICE void fold_tile(RowState<D, NT> &st, uint32_t kt, const QueryFrags<
       for (int i = 0; i < 2; ++i) {
         float &w0 = w[kb][i][0], &w1 = w[kb][i][1];
         w0 = s[kb][n][2 * i], w1 = s[kb][n][2 * i + 1];
-        add2(w0, w1, -mu[0], -mu[1]);
+        add2(w0, w1, up[0], up[1]);
         w0 = ex2_approx_ftz(w0), w1 = ex2_approx_ftz(w1);
         add2(st.l[n][0], st.l[n][1], w0, w1);
         if constexpr (C::kQuant) {

@@ -8,7 +8,8 @@
 //   * warp 5, one lane: S = Q K^T (128 x 64, fp32, one of two TMEM buffers), later O += P V (128 x D, fp32, TMEM), with
 //     P read from TMEM, where it overwrites its S;
 //   * warps 0-3, one thread per row: the running softmax. The maximum that weights refer to moves only when a row exceeds
-//     it by 2^8 (weights stay below 2^9, in range for fp16), so O is rarely rescaled; the sums are fp32.
+//     it by 2^8, so O is rarely rescaled; the sums are fp32. fp16 weights are held 2^kWeightUp times as large (why: see
+//     cache_attention.cu), at most 2^14.
 // 16-bit caches: two CTAs share an SM (113 KB of shared memory and 256 TMEM columns each), the one computes while the other
 // waits; 8-bit caches: one, with deeper rings. The grid is what the GPU holds at once, and each CTA takes an even share of the batch's tiles (cache_attention.cuh); the
 // roles walk the CTA's segments independently, so the loads of a segment start while the one before is finished.
@@ -28,6 +29,7 @@ constexpr int kTileRows = 128;
 constexpr int kTmemCols = 256;  // S: 2 x 64, O: up to 128
 constexpr int kColO = 128;
 constexpr int kPrefetch = 5;  // tiles ahead of the one being loaded that are brought into the L2
+constexpr float kWeightUp = 6.f;
 constexpr int kMinTiles = 4;  // of a CTA, where there are too few for all
 
 template <int CT, int D> struct Wide {
@@ -662,7 +664,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
         top *= rs;  // the tile's largest score
         const float mt = fmaxf(m, top);
         // The weights' reference M. While the row scales of V stay within 2^8 of each other it is the running maximum plus
-        // the bound of the largest one: no weight exceeds it, and fp16 holds the smallest ones' weights to 2^-17 of it. Once
+        // the bound of the largest one: no weight exceeds it, and fp16 holds the smallest ones' weights to 2^-23 of them. Once
         // they do not, and in tiles with keys that a row may not see (and must not notice), it is the row's own maximum of
         // score + bound.
         float Mt = M;
@@ -709,6 +711,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
           }
         }
         const float mu = m == -INFINITY ? 0.f : m;
+        const float up = (C::kBf16Mma ? 0.f : kWeightUp) - mu;
         const float cw = W::kQuant ? ex2_approx_ftz(mu - (M == -INFINITY ? 0.f : M)) : 1.f;
         uint64_t sum0 = 0, sum1 = 0;  // pairs of fp32
 #pragma unroll 1
@@ -721,7 +724,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
             for (int c = 0; c < 32; c += 4) {
               float w[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = ex2_approx_ftz(fmaf(x[h0 + c + e], rs, -mu));
+              for (int e = 0; e < 4; ++e) w[e] = ex2_approx_ftz(fmaf(x[h0 + c + e], rs, up));
               sum0 = f32x2_add(sum0, f32x2_pack(w[0], w[1])), sum1 = f32x2_add(sum1, f32x2_pack(w[2], w[3]));
               if constexpr (W::kQuant) {
                 const float4 v4 = sc[(kTileKeys + c0) / 4 + c / 4];

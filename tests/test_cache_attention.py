@@ -865,3 +865,46 @@ def test_the_largest_tree_with_every_value_infinite(cuda, cdt, bs):
     assert nanovllm_b200.status(cuda) == 0
     hit = got.isnan() if cdt == E4M3 else got == float("inf")
     assert bool(hit[0, 7].all()) and int(hit.sum()) == d and not bool(got[~hit].any())
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# A key that takes almost the whole softmax, over a long context.
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qdt,cdt", [(B16, B16), (H16, H16), (B16, E4M3), (H16, I8)])
+@pytest.mark.parametrize("B,n,splits", [(1, 1, 0), (1, 1, 5), (1, 12, 0), (1, 70, 0), (1300, 1, 0), (320, 70, 0)])
+@pytest.mark.parametrize("gap", [23.6, 26.0, 29.3])
+def test_many_small_weights_beside_a_large_one(cuda, qdt, cdt, B, n, splits, gap):
+    """The first key's score is `gap` binades above those of 20000 others, and its value is zero: the output is what the small
+    weights leave. Types of 16 bits hold weights relative to the largest one or two binades above it; fp16, whose step is
+    2^-24 from 2^-14 down, must have them far enough up. Both kernels keep the largest weight at 2^5 or above (2^13 in the
+    warp-level one), so a weight is off by 2^-30 of it at most, and half a step of its own type. Batches (of one sequence
+    over and over), so that a warp or a CTA holds much of a sequence."""
+    import nanovllm_b200
+    L, hq, d, bs = 20000, 2, 64, 64
+    g = torch.Generator().manual_seed(1)
+    pages = -(-L // bs)
+    table = torch.arange(pages, dtype=torch.int32)[None]
+    k, v = torch.zeros(pages, bs, 1, d), torch.randint(64, 128, (pages, bs, 1, d), generator=g).float()
+    k[0, 0, 0, 0], v[0, 0] = 64.0, 0.0
+    kv = [x.to(cdt) for x in (k, v)]
+    cache = [x.to(cuda) for x in kv]
+    kw = {}
+    if cdt in (E4M3, I8):
+        scale = torch.full((pages, 1, bs), 1.0 / 64)
+        kw = dict(k_scale=scale.to(cuda), v_scale=scale.to(cuda))
+        kv = [cm.row_values(x, scale) for x in kv]
+    q = torch.zeros(1, n, hq, d, dtype=qdt)
+    q[..., 0] = 1.0
+    of_batch = lambda x: x.expand(B, *x.shape[1:]).to(cuda)  # noqa: E731
+    top = 1.0 if cdt in (E4M3, I8) else 64.0
+    got = nanovllm_b200.tree_attention(of_batch(q), *cache, torch.full((B,), L, dtype=torch.int32, device=cuda), None,
+                                       of_batch(table), softmax_scale=gap * 0.6931471805599453 / top, num_splits=splits, **kw)
+    ref, spread, reach = cm.cache_attention(q, kv[0], kv[1], [L], table, None, [n], gap * 0.6931471805599453 / top)
+    u, uw = (2.0 ** -8 if t == B16 else 2.0 ** -11 for t in (qdt, cdt))
+    tol = u * ref.abs() + spread * (uw + 2.0 ** -18 + 2 * (d + 8) * 2.0 ** -24 * reach)
+    if cdt != B16:
+        tol = tol + 2.0 ** -30 * L * float(kv[1].double().abs().max())
+    assert float(ref.min()) > 0 and float((tol / ref).max()) < 1
+    err = (got.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), float((err / ref).max())
