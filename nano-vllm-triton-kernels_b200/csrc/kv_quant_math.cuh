@@ -4,8 +4,7 @@
 //   e4m3: scale = 2^E with E the smallest integer >= -126 for which a <= 448 * 2^E; code = x * 2^-E rounded to e4m3.
 //     A power of two, because the scaling is then exact: each code is ONE rounding of its element (half a step of
 //     2^-4 relative at most), and e4m3 being a floating format, up to one binade of unused headroom costs no precision.
-//   int8: scale = d / 127 with d = max(a, 127 * 2^-126); code = 127 x / d rounded half to even. 127 x is exact in fp32
-//     for bf16 and fp16 inputs and the quotient is the correctly rounded one, so the code is that of exact arithmetic.
+//   int8: scale = d / 127 with d = max(a, 127 * 2^-126); code = 127 x / d rounded half to even, as in exact arithmetic.
 //   A row that holds an infinity or NaN gets scale NaN and codes 0, so it reads back as NaN throughout.
 #pragma once
 
@@ -54,10 +53,22 @@ template <int FMT> NVB200_DEVICE RowScale row_scale(uint32_t amax_bits) {
   return r;
 }
 
-// int8: the code by the correctly rounded quotient, in the low byte.
-NVB200_DEVICE uint32_t exact_code(float x, const RowScale &r) {
-  return static_cast<uint32_t>(__float2int_rn(__fdiv_rn(__fmul_rn(x, r.mul), r.den)));
+// int8: the code of exact arithmetic, in the low byte. p: 127 x / d to within an eighth. The code's magnitude is n = floor(|p|)
+// or n + 1, by the sign of 127 |x| - (n + 1/2) d: the product is taken as hi + lo, exactly, and next to the middle the
+// difference of hi and (n + 1/2) d is one fp32 number (its unit is 2^-25 of d or more), so the sum's sign is the true one.
+NVB200_DEVICE uint32_t exact_code(float x, float p, const RowScale &r) {
+  const float ax = fabsf(x), n = floorf(fabsf(p));
+  const float hi = __fmul_rn(ax, r.mul), lo = __fmaf_rn(ax, r.mul, -hi);
+  const float side = __fadd_rn(__fmaf_rn(-(n + 0.5f), r.den, hi), lo);
+  const int k = static_cast<int>(n);
+  const int code = side > 0.f || (side == 0.f && (k & 1)) ? k + 1 : k;
+  return static_cast<uint32_t>(x < 0.f ? -code : code);
 }
+// Sums of this and a number of magnitude below 2^22 are rounded at the unit, half to even, and have it in the low bits.
+constexpr float kCodeMagic = 12582912.f;  // 1.5 * 2^23
+// A product x * (127 / d) as near as this to the middle between two codes says nothing of the code: its own rounding and the
+// quotient's move a value of at most 127 by less than 3 * 127 * 2^-24.
+constexpr float kCodeNear = 127.f * 2.384185791015625e-7f;  // 127 * 2^-22
 
 // Eight elements to eight codes, element 0 in the lowest byte.
 template <int FMT> NVB200_DEVICE uint2 quantise8(const float (&x)[8], const RowScale &r) {
@@ -67,21 +78,18 @@ template <int FMT> NVB200_DEVICE uint2 quantise8(const float (&x)[8], const RowS
     out.x = pack_e4m3x2(x[0] * r.mul, x[1] * r.mul) | pack_e4m3x2(x[2] * r.mul, x[3] * r.mul) << 16;
     out.y = pack_e4m3x2(x[4] * r.mul, x[5] * r.mul) | pack_e4m3x2(x[6] * r.mul, x[7] * r.mul) << 16;
   } else {
-    // x times the row's 127 / d, rounded at the unit by adding 1.5 * 2^23 (the code is then the sum's low byte). Two
-    // roundings of 2^-24 and the quotient's own move a value of at most 127 by less than 3 * 127 * 2^-24 < kNear, so
-    // where no product lies that near to the middle between two codes, they are the quotient's codes; else it is taken.
-    constexpr float kMagic = 12582912.f, kNear = 127.f * 2.384185791015625e-7f;  // 2^-22
+    // x times the row's 127 / d, rounded, where no product lies near the middle between two codes; else the exact codes.
     uint32_t c[8];
     float off = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float p = __fmul_rn(x[i], r.quot), m = __fadd_rn(p, kMagic);
-      off = fmaxf(off, fabsf(__fsub_rn(p, __fsub_rn(m, kMagic))));
+      const float p = __fmul_rn(x[i], r.quot), m = __fadd_rn(p, kCodeMagic);
+      off = fmaxf(off, fabsf(__fsub_rn(p, __fsub_rn(m, kCodeMagic))));
       c[i] = __float_as_uint(m);
     }
-    if (off > 0.5f - kNear) {
+    if (off > 0.5f - kCodeNear) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = exact_code(x[i], r);
+      for (int i = 0; i < 8; ++i) c[i] = exact_code(x[i], __fmul_rn(x[i], r.quot), r);
     }
     out.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     out.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
@@ -95,7 +103,7 @@ template <int FMT> NVB200_DEVICE uint8_t quantise1(float x, const RowScale &r) {
   if constexpr (FMT == kCacheE4M3)
     return static_cast<uint8_t>(pack_e4m3x2(x * r.mul, 0.f) & 0xFFu);
   else
-    return static_cast<uint8_t>(exact_code(x, r) & 0xFFu);
+    return static_cast<uint8_t>(exact_code(x, __fmul_rn(x, r.quot), r) & 0xFFu);
 }
 
 // Two e4m3 codes (low byte first) as two fp16 values: exact, every e4m3 value is an fp16 value.

@@ -464,3 +464,31 @@ def test_fused_many_tokens_equals_its_two_steps(cuda, fmt, T, hq, hkv, d):
     assert torch.equal(q1, q2) and torch.equal(k1, k2)
     _same(a, [_bits(t).cpu() for t in b])
     assert nanovllm_b200.status(cuda) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [128, 12])
+def test_int8_codes_of_fp32_rows_next_to_ties(cuda, d):
+    """fp32 elements at and next to the middle between two codes, for maxima of every size: the code is that of exact
+    arithmetic, in the vector kernel and the scalar one. (In 64 bits 127 x is exact, and no quotient of an fp32 pair lies within
+    2^-32 of a middle that it does not hit, so the oracle's is.)"""
+    import nanovllm_b200
+    T, hkv, bs = 600, 2, 16
+    g = torch.Generator().manual_seed(d)
+    top = torch.rand(T, hkv, 1, generator=g, dtype=torch.float64) + 1
+    e = torch.randint(-126, 127, (T, hkv, 1), generator=g).double()
+    e[::3] = torch.randint(-4, 5, e[::3].shape, generator=g).double()
+    top[::5] = 127 / 64  # exact middles
+    top = (top * torch.exp2(e)).float().clamp(min=127 * 2.0 ** -126).double()
+    k = torch.randint(0, 127, (T, hkv, d), generator=g).double() + 0.5
+    x = (k * top / 127).float()
+    bits = x.view(torch.int32) + torch.randint(-1, 2, x.shape, generator=g).int()
+    x = bits.view(torch.float32) * (1 - 2 * torch.randint(0, 2, x.shape, generator=g))
+    x = torch.minimum(torch.maximum(x, -top.float()), top.float())
+    x[..., 0] = top[..., 0].float()
+    pages = -(-T // bs)
+    cache = _cache(pages, bs, hkv, d, I8, cuda)
+    slots = torch.randperm(pages * bs, generator=g)[:T]
+    want = _expect_store(cache, x, -x, slots, bs)
+    nanovllm_b200.store_kvcache_quant(x.to(cuda), -x.to(cuda), *cache, slots.to(cuda))
+    _same(cache, want)
