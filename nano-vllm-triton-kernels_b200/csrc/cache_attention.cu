@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, Form<CT, D, NT, CLUSTER>::kCtasPerSm
   int u1, T = 0, ctas = 0;
   if constexpr (CLUSTER) {
     const int row_blocks = (p.rows + G::kRows - 1) / G::kRows;
-    const int b = blockIdx.z, rank = p.splits > 1 ? static_cast<int>(cta_rank_in_cluster()) : 0;
+    const int b = p.first_batch + blockIdx.z, rank = p.splits > 1 ? static_cast<int>(cta_rank_in_cluster()) : 0;
     const int h = blockIdx.y / row_blocks, block = blockIdx.y - h * row_blocks;
     // The queries' loads and the block table's first lines do not wait for the length, nor behind the keys' loads.
     load_q(b, h, block * G::kRows);
@@ -823,11 +823,17 @@ template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_s
   }
   static std::atomic<uint64_t> ready{0};
   if (int rc = allow_smem(cache_attention_kernel<CT, D, NT, true>, Cluster::kSmem, ready)) return rc;
-  if (n.units > 65535 || p.batch > 65535) return NVB200_ERR_UNSUPPORTED;
+  if (n.units > 65535) return NVB200_ERR_UNSUPPORTED;
   p.splits = num_splits > 0 ? num_splits
                             : cluster_splits(p, n.units * p.batch, kWarps * G::kTile, Cluster::kCtasPerSm);
-  return launch_ex(cache_attention_kernel<CT, D, NT, true>, dim3(p.splits, static_cast<unsigned>(n.units), p.batch),
-                   dim3(kThreads), Cluster::kSmem, s, p.splits, false, p);
+  constexpr int kMaxBatch = 65535;  // of a grid
+  for (int64_t b = 0; b < p.batch; b += kMaxBatch) {
+    p.first_batch = static_cast<int>(b);
+    const dim3 grid(p.splits, static_cast<unsigned>(n.units), static_cast<unsigned>(std::min<int64_t>(kMaxBatch, p.batch - b)));
+    if (int rc = launch_ex(cache_attention_kernel<CT, D, NT, true>, grid, dim3(kThreads), Cluster::kSmem, s, p.splits, false, p))
+      return rc;
+  }
+  return NVB200_OK;
 }
 
 // Whether a call takes the wide kernel (128 rows a CTA on the 5th-generation tensor cores) rather than blocks of 16 rows of

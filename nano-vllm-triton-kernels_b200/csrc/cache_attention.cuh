@@ -39,6 +39,7 @@ struct CacheAttnParams {
   int n, hq, hkv, group, block_size, bs_shift, max_pages, rows, causal;
   int batch;
   int splits;      // CTAs of a cluster sharing the keys of a sequence (cluster form)
+  int first_batch; // sequence of the grid's first (cluster form: a grid has at most 65535)
   // Workspace of the even-share form: what each CTA says of the start of its range, then [2 * grid] records of
   // [block_rows][D + 4] floats.
   struct CutInfo *cuts;

@@ -908,3 +908,32 @@ def test_many_small_weights_beside_a_large_one(cuda, qdt, cdt, B, n, splits, gap
     assert float(ref.min()) > 0 and float((tol / ref).max()) < 1
     err = (got.double().cpu() - ref).abs()
     assert bool((err <= tol).all()), float((err / ref).max())
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Limits.
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cdt", [B16, I8])
+@pytest.mark.parametrize("splits", [0, 2])
+def test_more_sequences_than_a_grid_holds(cuda, cdt, splits):
+    """65600 sequences: the bits of the same sequences in a call of their own, and the oracle's values on both sides of the
+    65535th."""
+    import nanovllm_b200
+    B, n, hq, hkv, d, bs = 65600, 2, 2, 1, 64, 16
+    g = torch.Generator().manual_seed(0)
+    q, kv, cache, table, _, _ = _problem(30, n, [20] * 30, hq, hkv, d, bs, B16, cdt, cuda, mask=None)
+    q = torch.randn(B, n, hq, d, generator=g).to(B16)
+    table = torch.randint(0, cache[0].shape[0], (B, 2), generator=g).int()
+    lens, drafts = (torch.randint(0, hi, (B,), generator=g).int() for hi in (33, 3))
+    mask = torch.rand(B, n, n, generator=g) < 0.5
+    dev = [x.to(cuda) for x in (q, lens, mask, table, drafts)]
+    run = lambda at: nanovllm_b200.tree_attention(  # noqa: E731
+        dev[0][at], cache[0], cache[1], dev[1][at], dev[2][at], dev[3][at], dev[4][at], k_scale=cache[2], v_scale=cache[3],
+        num_splits=splits)
+    nanovllm_b200.status(cuda, clear=True)
+    got = run(slice(None))
+    assert nanovllm_b200.status(cuda) == 0
+    assert torch.equal(got[:40000], run(slice(0, 40000))) and torch.equal(got[40000:], run(slice(40000, B)))
+    at = list(range(65520, 65550)) + [0, 1, B - 1]
+    _check(got[at], q[at], kv, table[at], lens[at].tolist(), mask[at], drafts[at].tolist(), d ** -0.5, cdt)
