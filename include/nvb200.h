@@ -403,7 +403,9 @@ NVB200_API int nvb200_load_kvcache_quant(void *key, void *value, const nvb200_qu
  *     entry lies outside [0, num_blocks) are seen by no row; they, lengths beyond max_blocks_per_seq * block_size
  *     and draft_lens outside [0, n] (both clamped) set NVB200_STATUS_BAD_SLOT.
  *   out: [batch, n, num_q_heads, head_dim] contiguous, dtype, written.
- * Takes head_dim 64 and 128, n <= 4096 and 16-byte aligned cache rows; NVB200_ERR_UNSUPPORTED otherwise.
+ * Takes head_dim 64 and 128, n <= 4096, rows = n * num_q_heads / num_kv_heads <= 65536, max_blocks_per_seq * block_size <=
+ * 2^31 - 65536 and 16-byte aligned cache rows, any batch; where the sizes or strides leave it to the kernel for few rows
+ * (num_splits > 0, pages not a multiple of 8 tokens), num_kv_heads * ceil(rows / 16) <= 65535. NVB200_ERR_UNSUPPORTED otherwise.
  * Replaces: nothing in the reference, which verifies linear drafts through flash_attn_with_kvcache
  * (nanovllm/layers/attention.py:84-91). */
 typedef struct nvb200_cache_attention_args {

@@ -796,6 +796,7 @@ int64_t total_tiles(const CacheAttnParams &p, const NarrowShape &n) {
 // few (32 sequences of 1024 keys: 17.4 against 25.2 us), where the units fill several waves, and for one sequence, unless it
 // has too few CTAs in its clusters (24 sequences of up to 32768 keys: 197 against 239 us).
 constexpr int kFewKeys = 2048;
+constexpr int64_t kMaxUnits = 65535;  // of a sequence, in the cluster form's grid
 int narrow_grid(const CacheAttnParams &p, const NarrowShape &n, int num_splits) {
   if (num_splits > 0) return 0;
   const int64_t units = n.units * p.batch, slots = static_cast<int64_t>(n.ctas_per_sm) * sm_count();
@@ -823,7 +824,7 @@ template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_s
   }
   static std::atomic<uint64_t> ready{0};
   if (int rc = allow_smem(cache_attention_kernel<CT, D, NT, true>, Cluster::kSmem, ready)) return rc;
-  if (n.units > 65535) return NVB200_ERR_UNSUPPORTED;
+  if (n.units > kMaxUnits) return NVB200_ERR_UNSUPPORTED;
   p.splits = num_splits > 0 ? num_splits
                             : cluster_splits(p, n.units * p.batch, kWarps * G::kTile, Cluster::kCtasPerSm);
   constexpr int kMaxBatch = 65535;  // of a grid
@@ -913,7 +914,8 @@ extern "C" int64_t nvb200_cache_attention_workspace_size(const nvb200_cache_atte
   if (!launch) return 0;
   if (prefers_wide(p, ct) && a->num_splits == 0 && wide_takes(p)) return wide_workspace_bytes(p, ct, a->head_dim);
   const NarrowShape n = narrow_shape(p, ct, a->head_dim);
-  return even_share_bytes(narrow_grid(p, n, a->num_splits), n.rows, a->head_dim);
+  const int grid = narrow_grid(p, n, a->num_splits);
+  return grid == 0 && n.units > kMaxUnits ? -1 : even_share_bytes(grid, n.rows, a->head_dim);
 }
 
 extern "C" int nvb200_cache_attention(const nvb200_cache_attention_args *a, void *workspace, int64_t workspace_bytes,
@@ -924,8 +926,9 @@ extern "C" int nvb200_cache_attention(const nvb200_cache_attention_args *a, void
   if (int rc = prepare_attention(a, p, &ct, &launch)) return rc;
   if (!launch) return NVB200_OK;
   if (workspace_bytes < 0 || !aligned16(workspace)) return NVB200_ERR_ARG;
-  if (int rc = check_device()) return rc;
   const int64_t need = nvb200_cache_attention_workspace_size(a);
+  if (need < 0) return NVB200_ERR_UNSUPPORTED;
+  if (int rc = check_device()) return rc;
   if (workspace && workspace_bytes < need) return NVB200_ERR_ARG;
   if (need == 0) workspace = nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

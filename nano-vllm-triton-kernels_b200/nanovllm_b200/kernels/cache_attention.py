@@ -18,6 +18,7 @@ from nanovllm_b200.kernels.kv_quant import check_quant_cache
 
 _QUERY = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 MAX_NEW_TOKENS = 4096
+MAX_ROWS = 65536  # query rows per KV head
 
 
 def _require(cond: bool, msg: str = "") -> None:
@@ -52,6 +53,8 @@ def _run(what, q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table
         raise NotImplementedError(f"{what}: head_dim must be 64 or 128")
     if n > MAX_NEW_TOKENS:
         raise NotImplementedError(f"{what}: at most {MAX_NEW_TOKENS} new tokens per sequence")
+    if n * (hq // hkv) > MAX_ROWS:
+        raise NotImplementedError(f"{what}: at most {MAX_ROWS} query rows (n * Hq / Hkv) per KV head")
     _require(0 <= num_splits <= 8, "num_splits must be 0 (automatic) to 8")
     _require(cache_seqlens.shape == (B,) and cache_seqlens.dtype == torch.int32, "cache_seqlens must be int32 [B]")
     _require(k_cache.get_device() == v_cache.get_device() == cache_seqlens.get_device() == idx,
@@ -98,8 +101,8 @@ def _run(what, q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
         rc = L.nvb200_cache_attention(a, _lib.ptr(ws), max(need, 0), _lib.stream_of(q))
     if rc == _lib.ERR_UNSUPPORTED:
-        raise NotImplementedError(f"{what}: cache rows must be 16-byte aligned, and a sequence's block table address "
-                                  "fewer than 2^31 - 65536 keys")
+        raise NotImplementedError(f"{what}: cache rows must be 16-byte aligned, a sequence's block table address at most "
+                                  "2^31 - 65536 keys, and Hkv * ceil(n * Hq / Hkv / 16) be at most 65535")
     _lib.check(rc, what)
     return out
 

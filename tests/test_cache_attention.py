@@ -913,6 +913,32 @@ def test_many_small_weights_beside_a_large_one(cuda, qdt, cdt, B, n, splits, gap
 # ---------------------------------------------------------------------------------------------------------------
 # Limits.
 
+def test_limits_are_refused_by_size_and_call_alike():
+    """workspace_size says -1 for sizes that the call refuses, whatever form they would take."""
+    from nanovllm_b200 import _lib
+    L = _lib.lib()
+    for kw in (dict(queries_per_seq=4096, num_q_heads=17), dict(queries_per_seq=4097), dict(max_blocks_per_seq=(1 << 25)),
+               # 16 x 4096 blocks of 16 rows, kept from the many-row kernel by its split count, its page size or its alignment
+               dict(queries_per_seq=4096, num_q_heads=256, num_kv_heads=16, num_splits=1),
+               dict(queries_per_seq=4096, num_q_heads=256, num_kv_heads=16, block_size=12),
+               dict(queries_per_seq=4096, num_q_heads=256, num_kv_heads=16, k_scale=(1 << 20) + 4)):
+        a = _host_args(**kw)
+        assert L.nvb200_cache_attention_workspace_size(a) == -1, kw
+        assert L.nvb200_cache_attention(a, None, 0, None) == _lib.ERR_UNSUPPORTED, kw
+    for kw in (dict(queries_per_seq=4096, num_q_heads=16), dict(queries_per_seq=4096, num_q_heads=256, num_kv_heads=16),
+               dict(batch=1 << 20), dict(batch=1 << 20, num_splits=3)):
+        assert L.nvb200_cache_attention_workspace_size(_host_args(**kw)) >= 0, kw
+
+
+@pytest.mark.gpu
+def test_row_limit_is_named(cuda):
+    import nanovllm_b200
+    q = torch.zeros(1, 4096, 17, 64, dtype=B16, device=cuda)
+    kc = torch.zeros(1, 64, 1, 64, dtype=B16, device=cuda)
+    with pytest.raises(NotImplementedError, match="65536 query rows"):
+        nanovllm_b200.tree_attention(q, kc, kc, torch.ones(1, dtype=torch.int32, device=cuda))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("cdt", [B16, I8])
 @pytest.mark.parametrize("splits", [0, 2])
