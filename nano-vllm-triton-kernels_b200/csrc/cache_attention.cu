@@ -7,7 +7,8 @@
 //   s_j = scale * ks_j * (q . k_j),  p_j = 2^(s_j log2 e - m),  out = (sum_j p_j vs_j v_j) / (sum_j p_j)
 // with k_j, v_j the stored codes and ks_j, vs_j their row scales (1 for 16-bit caches); one pass over the keys with the
 // running maximum m and sum l. Masked keys are selected away (p = 0 by selection, never by adding -inf), so no value of
-// a key that a row does not see, infinities and NaN included, reaches it; a row that sees no key gives zeros.
+// a key that a row does not see, infinities and NaN included, reaches it; a row that sees no key gives zeros. A weight below
+// fp32's normal range, 2^-126 of the row's largest, is zero, whatever its value's scale.
 //
 // 8-bit caches run on fp16 matrix instructions: e4m3 and int8 codes are exact in fp16 (one conversion per two codes), and
 // the query row is brought to fp16 by an exact power of two, so the only roundings are those of p and the output.
