@@ -56,6 +56,8 @@ def _run(what, q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table
     if n * (hq // hkv) > MAX_ROWS:
         raise NotImplementedError(f"{what}: at most {MAX_ROWS} query rows (n * Hq / Hkv) per KV head")
     _require(0 <= num_splits <= 8, "num_splits must be 0 (automatic) to 8")
+    if isinstance(cache_seqlens, int):
+        cache_seqlens = torch.full((B,), cache_seqlens, dtype=torch.int32, device=dev)
     _require(cache_seqlens.shape == (B,) and cache_seqlens.dtype == torch.int32, "cache_seqlens must be int32 [B]")
     _require(k_cache.get_device() == v_cache.get_device() == cache_seqlens.get_device() == idx,
              "q, the caches and cache_seqlens must be on one device")
@@ -114,8 +116,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                    num_splits: int = 0) -> torch.Tensor:
     """q: [B, n, Hq, D] bf16 or fp16, the new tokens of B sequences. k_cache, v_cache: [blocks, block_size, Hkv, D] (with
     block_table [B, max_blocks] int32) or [B, max_len, Hkv, D] (without), in q's dtype, or 8-bit with k_scale, v_scale
-    [blocks, Hkv, block_size]. cache_seqlens: [B] int32, the keys in the cache per sequence, the new tokens being the last
-    draft_lens[b] of them ([B] int32, default n).
+    [blocks, Hkv, block_size]. cache_seqlens: [B] int32 or an int, the keys in the cache per sequence, the new tokens being
+    the last draft_lens[b] of them ([B] int32, default n).
     tree_mask: bool [n, n] or [B, n, n]; new token i sees the context (the keys before the new tokens) and new token j
     where tree_mask[..., i, j] (nothing is implied: a token sees itself only if its mask says so). None: the chain, token i
     sees new tokens 0..i. Returns [B, n, Hq, D] in q's dtype; tokens i >= draft_lens[b], and rows that see no key, give
@@ -129,7 +131,7 @@ def decode_attention_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                            v_scale: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor | None = None,
                            softmax_scale: float | None = None, causal: bool = False, num_splits: int = 0) -> torch.Tensor:
     """`attention.decode_attention` over an 8-bit cache (kv_quant): q [B, n, Hq, D] bf16 or fp16 against the
-    cache_seqlens[b] keys of each sequence; causal aligns query i of n with key L - n + i. Returns [B, n, Hq, D]."""
+    cache_seqlens[b] keys of each sequence ([B] int32, or an int for all); causal aligns query i of n with key L - n + i. Returns [B, n, Hq, D]."""
     _require(k_scale is not None and v_scale is not None, "decode_attention_quant: an 8-bit cache has scales")
     return _run("decode_attention_quant", q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, None, None,
                 softmax_scale, causal, num_splits)

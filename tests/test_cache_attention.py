@@ -963,3 +963,18 @@ def test_more_sequences_than_a_grid_holds(cuda, cdt, splits):
     assert torch.equal(got[:40000], run(slice(0, 40000))) and torch.equal(got[40000:], run(slice(40000, B)))
     at = list(range(65520, 65550)) + [0, 1, B - 1]
     _check(got[at], q[at], kv, table[at], lens[at].tolist(), mask[at], drafts[at].tolist(), d ** -0.5, cdt)
+
+
+@pytest.mark.gpu
+def test_one_length_for_all_sequences(cuda):
+    """cache_seqlens as an int, as the 16-bit decode attention takes it."""
+    import nanovllm_b200
+    q, kv, cache, table, m, drafts = _problem(3, 2, [37] * 3, 4, 2, 64, 16, B16, E4M3, cuda)
+    got = nanovllm_b200.decode_attention_quant(q.to(cuda), *cache, 37, table.to(cuda), causal=True)
+    _check(got, q, kv, table, [37] * 3, None, drafts, 64 ** -0.5, E4M3)
+    got = nanovllm_b200.tree_attention(q.to(cuda), cache[0], cache[1], 37, m.to(cuda), table.to(cuda), k_scale=cache[2],
+                                       v_scale=cache[3])
+    _check(got, q, kv, table, [37] * 3, m, drafts, 64 ** -0.5, E4M3)
+    nanovllm_b200.status(cuda, clear=True)
+    nanovllm_b200.decode_attention_quant(q.to(cuda), *cache, 49, table.to(cuda))  # a key more than the table holds
+    assert nanovllm_b200.status(cuda, clear=True) == 2
