@@ -355,7 +355,7 @@ typedef struct nvb200_quant_cache {
  * s % block_size of block s / block_size). Slot -1 stores nothing; a slot outside [-1, num_blocks * block_size) is not
  * stored and sets NVB200_STATUS_BAD_SLOT. The other slots of one call must differ from each other: two tokens written
  * to one slot leave its codes and scale from different tokens. dtype: of key and value. Any head_dim and alignment;
- * multiples of 8 up to 256 on 16-byte aligned rows take the vectorised kernel.
+ * multiples of 16 up to 512 on 16-byte aligned rows take the vectorised kernel.
  * Counterpart in the reference: nanovllm/layers/attention.py:34-41 (store_kvcache), 16-bit only. */
 NVB200_API int nvb200_store_kvcache_quant(const void *key, int64_t key_token_stride, const void *value,
                                           int64_t value_token_stride, const void *slot_mapping, int slot_bytes,

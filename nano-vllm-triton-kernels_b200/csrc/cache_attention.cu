@@ -794,8 +794,10 @@ int64_t total_tiles(const CacheAttnParams &p, const NarrowShape &n) {
 
 // CTAs of the even-share form; 0: the call takes the cluster form, one launch instead of two, whose CTAs of one sequence are
 // even but whose sequences may not be. That costs at most one sequence's keys, so it stays where the block tables address
-// few (32 sequences of 1024 keys: 17.4 against 25.2 us), where the units fill several waves, and for one sequence, unless it
-// has too few CTAs in its clusters (24 sequences of up to 32768 keys: 197 against 239 us).
+// few (32 sequences of 1024 keys: 15.8 us; even shares 22.3), where the units fill several waves, and for one sequence, unless
+// it has too few CTAs in its clusters (24 sequences of up to 32768 keys: 268 us; even shares 200). The host knows the tables'
+// width, not the lengths: short sequences in wide tables take even shares too (the 32 x 1024 above in tables of 4096 keys
+// 22.2 us, 16.3 with num_splits = 1).
 constexpr int kFewKeys = 2048;
 constexpr int64_t kMaxUnits = 65535;  // of a sequence, in the cluster form's grid
 int narrow_grid(const CacheAttnParams &p, const NarrowShape &n, int num_splits) {
@@ -839,13 +841,19 @@ template <int CT, int D, int NT> int launch_narrow(CacheAttnParams &p, int num_s
 }
 
 // Whether a call takes the wide kernel (128 rows a CTA on the 5th-generation tensor cores) rather than blocks of 16 rows of
-// this one. Measured on B200, head_dim 128, group 4, this kernel / the wide one, us, for ragged batches of (sequences x keys):
-//   16-bit cache, 64 rows:  32 x 2048  79 /  75, 32 x 4096 182 / 109, 8 x 16384 144 /  94
+// this one: above 32 (16-bit) or 64 rows (8-bit) where the tables address many keys, above twice that elsewhere. Measured on
+// B200, head_dim 128, group 4, this kernel / the wide one, us, for ragged batches of (sequences x keys):
+//   16-bit cache, 40 and 48 rows: 32 x 2048  74 /  68, 80 / 74
+//   16-bit cache, 64 rows:  32 x 2048  78 /  77, 32 x 4096 182 / 109, 8 x 16384 144 /  94
 //   16-bit cache, 128 rows: 32 x 2048 151 /  94, 32 x 4096 225 / 118, 8 x 16384 271 / 110
 //   8-bit cache,  64 rows:  32 x 2048  70 / 129, 32 x 4096 133 / 183, 8 x 16384 105 / 144
-//   8-bit cache,  128 rows: 32 x 2048 132 / 147, 32 x 4096 241 / 223, 8 x 16384 213 / 148
+//   8-bit cache,  72, 96 and 112 rows: 32 x 2048 82 / 123, 98 / 153, 112 / 137
+//   8-bit cache,  128 rows: 32 x 2048 120 / 147, 32 x 4096 241 / 223, 8 x 16384 213 / 148
 //   8-bit cache,  256 rows: 4 x 2048   61 /  46, 8 x 16384 351 / 227
-// (8-bit tiles pass through shared memory twice there; long tables let its roles run undisturbed).
+// (8-bit tiles pass through shared memory twice there; long tables let its roles run undisturbed). The rule stands at measured
+// row counts, not at the crossings: up to 8 % is lost at 40 to 64 rows of 16-bit caches in short tables, and in long tables the
+// 8-bit lines cross somewhere between 64 and 128 rows. head_dim 64 has the same rule (32 x 2048: 16-bit 64 rows 51 / 58, 8-bit
+// 72 rows 54 / 100, 128 rows 85 / 112).
 bool prefers_wide(const CacheAttnParams &p, int ct) {
   const bool many_keys = static_cast<int64_t>(p.max_pages) * p.block_size > kFewKeys;
   const int few_rows = ct == kE4M3 || ct == kI8 ? 64 : 32;

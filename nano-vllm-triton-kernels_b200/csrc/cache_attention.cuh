@@ -270,8 +270,8 @@ NVB200_DEVICE int page_of(const CacheAttnParams &p, int j) {
 // Infinities and NaN of V among the new tokens are taken out of the tiles (0 * inf is NaN in a matrix instruction, and a
 // row may not see them); a row that does see one gets it from here, where it decides a column whatever its weight: what those
 // that token qi sees add to columns d .. d + N - 1 of KV head h (d a multiple of N: one piece of the row). Only for segments
-// that held one. The loads of eight keys are in flight together, so the scan of the largest call (4096 new tokens, 16 pieces
-// of a row) takes some milliseconds where a key at a time took a good part of the second that waiting warps allow.
+// that held one. The loads of eight keys are in flight together, so a call of 4096 new tokens with infinities in all
+// of them takes 3.2 ms (wide kernel, one KV head, head_dim 128; 0.09 ms without), far from the second that waiting warps allow.
 template <int N> struct Columns {
   float v[N];
 };

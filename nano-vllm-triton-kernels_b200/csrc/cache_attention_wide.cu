@@ -629,8 +629,10 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
           if (qi < 0) see = 0ull;
           see_lo = lo & static_cast<uint32_t>(see), see_hi = hi & static_cast<uint32_t>(see >> 32);
         }
-        // Scores of columns c0 .. c0 + CW before the row's factor rs > 0. 8-bit caches read S twice, 32 columns at a time (for the maximum, then for the weights): a tile's 64 scores beside three numbers per key do not fit
-        // the registers of a thread, and what is spilled goes to the L2, the L1 being all shared memory here.
+        // Scores of columns c0 .. c0 + CW before the row's factor rs > 0. 8-bit caches read S twice, 32 columns at a
+        // time (for the maximum, then for the weights; a third time where row scales lie far apart): a tile's 64 scores beside
+        // three numbers per key do not fit the registers of a thread, and what is spilled goes to the L2, the L1 being all
+        // shared memory here.
         constexpr int CW = W::kQuant ? 32 : 64;
         float x[CW];
         auto scores = [&](int c0) {

@@ -5,8 +5,8 @@
 // the writes, 4 bytes per row either way, are merged in the L2. kv_quant_math.cuh has the quantiser.
 //
 // All three are HBM-bound: every row is read once and written once, and a row's maximum is taken from registers, so
-// nothing is read a second time. A group of D / 16 lanes (a power of two of them) holds a row, 8 elements of each half a
-// lane: 16-byte loads of 16-bit inputs, 8-byte stores of codes, and the maximum by shuffles within the group.
+// nothing is read a second time. A group of 4 to 32 lanes, the power of two of D / 16 or the next above it (lanes past
+// D / 16 hold nothing), holds a row, 8 elements of each half a lane: 16-byte loads of 16-bit inputs, 8-byte stores of codes, and the maximum by shuffles within the group.
 #include <algorithm>
 #include <type_traits>
 
@@ -525,7 +525,7 @@ template <typename T, int FMT> int launch_load_quant(LoadQuantArgs &a, bool vec,
         <<<grid_for(2 * a.total * a.c.hkv, kQuantThreads / 32, 8), kQuantThreads, 0, s>>>(a);
     return launch_status();
   }
-  // Tokens a warp: 2 share a search's latency; more leave the last warps behind (176k tokens: 2 99 us, 4 103 us, 8 110 us).
+  // Tokens a warp: 2 share a search's latency; more leave the last warps behind (176k tokens of 8 heads: 2 99 us, 4 103 us, 8 110 us; fewer heads leave lanes without a row).
   const int64_t warps = static_cast<int64_t>(sm_count()) * 64;
   a.run = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2, a.total / warps)));
   const int64_t per_cta = static_cast<int64_t>(a.run) * (kQuantThreads / 32);
