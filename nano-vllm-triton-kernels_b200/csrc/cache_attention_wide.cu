@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
   if (tid == 0) {
     for (int i = 0; i < W::NK; ++i) mbar_init(b_kfull + 8 * i, W::kQuant ? W::kConvWarps : 1), mbar_init(b_kempty + 8 * i, 1);
     for (int i = 0; i < W::NV; ++i) mbar_init(b_vfull + 8 * i, W::kQuant ? W::kConvWarps : 1), mbar_init(b_vempty + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(b_sfull + 8 * i, 2), mbar_init(b_pready + 8 * i, 4), mbar_init(b_pv + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(b_sfull + 8 * i, 2), mbar_init(b_pready + 8 * i, 4), mbar_init(b_pv + 8 * i, 2);
     mbar_init(b_q, 4);
     for (int i = 0; i < W::NR; ++i) mbar_init(b_rfull + 8 * i, 1), mbar_init(b_rempty + 8 * i, W::kConvWarps);
     st_shared_u32(failed, 0u);
@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(Wide<CT, D>::kThreads, Wide<CT, D>::kCtas)
             tc_mma_ts(td + kColO, pa + k * 8, bd + k * (16 * 128 >> 4), idesc_o, (t > 0 || k > 0) ? 1u : 0u);
           tc_commit(b_vempty + 8 * st);
           tc_commit(b_pv + 8 * (i & 1));
+          mbar_arrive(b_pv + 8 * (i & 1));  // orders the marks of V's infinities (dirty_word), seen through b_vfull and b_pready
         }
         __syncwarp();
       }
